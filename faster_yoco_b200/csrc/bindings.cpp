@@ -84,6 +84,15 @@ std::vector<at::Tensor> retention_bwd(const at::Tensor& dout, const at::Tensor& 
                                       const c10::optional<at::Tensor>& dv_out,
                                       const c10::optional<at::Tensor>& rope_cos,
                                       const c10::optional<at::Tensor>& rope_sin);
+at::Tensor shared_prefix_attention(const at::Tensor& q, const at::Tensor& pk, const at::Tensor& pv,
+                                   const at::Tensor& k, const at::Tensor& v,
+                                   const c10::optional<at::Tensor>& lengths,
+                                   const c10::optional<at::Tensor>& prefix_lengths, double scale);
+std::vector<at::Tensor> sample(const at::Tensor& logits, const at::Tensor& u,
+                               const c10::optional<at::Tensor>& temperature, double temperature_all,
+                               const c10::optional<at::Tensor>& top_k, int64_t top_k_all,
+                               const c10::optional<at::Tensor>& top_p, double top_p_all,
+                               const c10::optional<at::Tensor>& min_p, double min_p_all, bool want_logprob);
 std::vector<at::Tensor> ipc_alloc(int64_t nbytes);
 int64_t ipc_open(const at::Tensor& handle_bytes);
 void ipc_close(int64_t ptr);
@@ -232,6 +241,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("retention_bwd", &fyb::retention_bwd, py::arg("dout"), py::arg("q"), py::arg("k"), py::arg("v"),
         py::arg("gcum"), py::arg("o"), py::arg("dq_out") = py::none(), py::arg("dk_out") = py::none(),
         py::arg("dv_out") = py::none(), py::arg("rope_cos") = py::none(), py::arg("rope_sin") = py::none());
+  m.def("shared_prefix_attention", &fyb::shared_prefix_attention,
+        "decode attention over a prefix shared by the rows of a group and each row's own keys", py::arg("q"),
+        py::arg("prefix_k"), py::arg("prefix_v"), py::arg("k"), py::arg("v"), py::arg("lengths"),
+        py::arg("prefix_lengths"), py::arg("scale"));
+  m.def("sample", &fyb::sample, "{token, log-probability} of each row of logits (temperature, top-k, top-p, min-p)");
   m.def("ipc_alloc", &fyb::ipc_alloc, "cudaMalloc'd byte buffer + its CUDA IPC handle");
   m.def("ipc_open", &fyb::ipc_open);
   m.def("ipc_close", &fyb::ipc_close);

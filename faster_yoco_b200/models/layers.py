@@ -313,9 +313,14 @@ class CrossAttention(nn.Module):
         self.q_proj = Linear(args.dim, args.dim, I.init_method, parallel="column")
         self.out_proj = Linear(args.dim, args.dim, I.init_method, parallel="row")
 
-    def forward(self, x, key, value, rel_pos, residual=None, q_offset: Optional[int] = None):
+    def forward(self, x, key, value, rel_pos, residual=None, q_offset: Optional[int] = None, prefix=None):
+        """prefix: (key, value) [G, P, heads, D] of prompts shared by the rows of each group; key / value then hold
+        the positions after it."""
         B, L, _ = x.shape
         q = ops.rope(self.q_proj(TP.copy_to_tp(x)).view(B, L, self.num_heads, self.head_dim), *rel_pos)
+        if prefix is not None:
+            o = ops.shared_prefix_attention(q, *prefix, key, value)
+            return self.out_proj(o.reshape(B, L, self.num_heads * self.head_dim), residual)
         if q_offset is None and CP.cp_size() > 1 and key.shape[1] == CP.cp_size() * L:
             q_offset = CP.cp_rank() * L              # this rank's block inside the gathered sequence
         if key.shape[1] != L:

@@ -62,14 +62,14 @@ class DecoderLayer(nn.Module):
                                              *common, cos, sin, cfg)
 
     def forward(self, x, start_pos=0, key=None, value=None, rel_pos=None, incremental_state=None,
-                is_prefilling=False):
+                is_prefilling=False, prefix=None):
         from .fused import fused_path_ok
         if incremental_state is None and self.training and fused_path_ok(x, self.mixer.head_dim):
             return self._fused(x, key, value, rel_pos)
         residual = x
         h = self.mixer_layer_norm(x)
         if self.is_cross_layer:
-            x = self.mixer(h, key, value, rel_pos=rel_pos, residual=residual)
+            x = self.mixer(h, key, value, rel_pos=rel_pos, residual=residual, prefix=prefix)
         elif self.args.sliding_window is not None:
             x = self.mixer(h, rel_pos=rel_pos, start_pos=start_pos, incremental_state=incremental_state,
                            residual=residual)
@@ -189,14 +189,21 @@ class CrossDecoder(nn.Module):
         key, value, rel_pos = self.shared_kv(x, start_pos, fused=fused)
         if cp:                                   # the one shared K / V over the whole sequence, for every layer
             key, value = CP.gather_seq(key, 1), CP.gather_seq(value, 1)
+        prefix = None
         if incremental_state is not None:
             st = incremental_state
+            if "prefix_key" in st:               # forked rows: the cache below holds the positions after the prefix
+                prefix = st["prefix_key"], st["prefix_value"]
+                start_pos = start_pos - prefix[0].shape[1]
+                if start_pos < 0:
+                    raise ValueError("a forked state continues behind its prefix: start_pos is inside it")
             need = start_pos + seqlen
             have = st["prev_key"].shape[1] if "prev_key" in st else 0
             if need > have:
                 # the shared KV cache holds max_seq_len positions; a longer prompt + generation grows it (the
                 # filled prefix is kept)
-                size = max(self.args.max_seq_len, (need + 1023) // 1024 * 1024)
+                size = (need + 255) // 256 * 256 if prefix is not None else \
+                    max(self.args.max_seq_len, (need + 1023) // 1024 * 1024)
                 shape = (bsz, size, self.num_heads, self.head_dim)
                 nk = torch.empty(shape, device=x.device, dtype=x.dtype)
                 nv = torch.empty(shape, device=x.device, dtype=x.dtype)
@@ -206,6 +213,7 @@ class CrossDecoder(nn.Module):
                 st["prev_key"], st["prev_value"] = nk, nv
             st["prev_key"][:, start_pos:start_pos + seqlen] = key
             st["prev_value"][:, start_pos:start_pos + seqlen] = value
+            st["filled"] = start_pos + seqlen
             key = st["prev_key"][:, :start_pos + seqlen]
             value = st["prev_value"][:, :start_pos + seqlen]
         if skip_cross_decoder:
@@ -219,7 +227,7 @@ class CrossDecoder(nn.Module):
                 x = torch.utils.checkpoint.checkpoint(layer, x, 0, key, value, rel_pos, None, False,
                                                       use_reentrant=False)
             else:
-                x = layer(x, key=key, value=value, rel_pos=rel_pos)
+                x = layer(x, key=key, value=value, rel_pos=rel_pos, prefix=prefix)
         return x
 
 
@@ -341,6 +349,29 @@ class YOCO(nn.Module):
         if return_hidden:
             return h, None
         return self.output_layer(h), None
+
+    @torch.no_grad()
+    def fork_state(self, state: Dict, batch: int, copies: int) -> Dict:
+        """The incremental state of ``batch * copies`` rows (row r continues prompt r // copies) from the state of
+        ``batch`` prefilled prompts: the self-decoder's states, which do not grow with the prompt, are copied; the one
+        shared K / V cache of the prompts becomes a prefix that the copies read in place, and each copy gets a cache
+        of its own for the positions after it."""
+        out: Dict = {}
+        for idx in range(len(self.self_decoder.layers)):
+            st = out[idx] = dict(state.get(idx, {}))
+            st.pop("index_mask", None)
+            for name in ("last_hidden_state", "prev_key", "prev_value"):
+                if st.get(name) is not None:
+                    st[name] = st[name][:batch].repeat_interleave(copies, 0)
+        cd, w = self.cross_decoder, self.output_projection.weight
+        if "prefix_key" in state:
+            raise ValueError("fork_state: the state is forked already")
+        n = state.get("filled", 0)
+        for name in ("key", "value"):
+            full = state.get("prev_" + name)
+            out["prefix_" + name] = (full[:batch, :n] if full is not None else
+                                     torch.empty(batch, 0, cd.num_heads, cd.head_dim, device=w.device, dtype=w.dtype))
+        return out
 
     def output_layer(self, features):
         return self.output_projection(features)

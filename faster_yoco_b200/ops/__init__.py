@@ -525,6 +525,116 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal: bool = 
     return ref.attention(q, k, v, causal=causal, window=window, q_offset=k.shape[1] - q.shape[1])
 
 
+def _no_grad_op(name: str, *tensors):
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+        raise RuntimeError(f"{name} has no backward pass: call it under torch.no_grad() or on detached tensors")
+
+
+def _vec16(t: torch.Tensor) -> torch.Tensor:
+    """t itself when its last dimension is contiguous and its rows start on 16-byte boundaries (2-byte types), else a
+    contiguous copy."""
+    if (t.stride(-1) == 1 and t.data_ptr() % 16 == 0
+            and all(st % 8 == 0 and st > 0 for st, n in zip(t.stride()[:-1], t.shape) if n > 1)):
+        return t
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def shared_prefix_attention(q: torch.Tensor, prefix_k: torch.Tensor, prefix_v: torch.Tensor, k: torch.Tensor,
+                            v: torch.Tensor, lengths: Optional[torch.Tensor] = None,
+                            prefix_lengths: Optional[torch.Tensor] = None,
+                            scale: Optional[float] = None) -> torch.Tensor:
+    """Decode attention of a batch whose rows share long prefixes that are stored, and read, once.
+
+    q: [B, Lq, Hq, D]; prefix_k / prefix_v: [G, P, Hk, D], group g serving rows g * (B // G) .. (g + 1) * (B // G) - 1;
+    k / v: [B, S, Hk, D], each row's own positions. Query i of row b sees the prefix keys j < prefix_lengths[g] and the
+    own keys j < lengths[b] with j <= lengths[b] - Lq + i (the causal diagonal ends at the last own key, as in
+    ``attention``). lengths [B] / prefix_lengths [G]: int32 or int64 on q's device, clamped to [0, S] / [0, P]; None
+    means all stored positions. Positions behind the lengths may hold anything. P, S, B or Lq may be 0; a query that
+    sees no key gets zeros. scale: default 1 / sqrt(D). Returns a contiguous [B, Lq, Hq, D].
+
+    The sm_100a kernel takes bf16 and fp16 with D 64 or 128 and at most 128 query heads a key / value head; other
+    types and sizes run the PyTorch expression. Key / value tensors are read in place when their rows are 16-byte
+    aligned, else copied first. A value that SOME query of a row sees has to be finite. Inference only."""
+    _no_grad_op("shared_prefix_attention", q, prefix_k, prefix_v, k, v)
+    kv = (prefix_k, prefix_v, k, v)
+    if any(t.dim() != 4 for t in (q, *kv)):
+        raise ValueError("shared_prefix_attention: q, prefix_k, prefix_v, k and v have four dimensions")
+    if any(t.dtype != q.dtype or t.device != q.device for t in kv):
+        raise ValueError("shared_prefix_attention: q, prefix_k, prefix_v, k and v must share a type and a device")
+    B, Lq, Hq, D = q.shape
+    G, P, Hk, _ = prefix_k.shape
+    if prefix_v.shape != prefix_k.shape or v.shape != k.shape or k.shape[0] != B or k.shape[2:] != prefix_k.shape[2:]:
+        raise ValueError(f"shared_prefix_attention: key / value shapes {tuple(prefix_k.shape)}, {tuple(prefix_v.shape)}, "
+                         f"{tuple(k.shape)}, {tuple(v.shape)} do not fit together")
+    if prefix_k.shape[3] != D or Hk == 0 or D == 0 or Hq % Hk or G == 0 or B % G:
+        raise ValueError(f"shared_prefix_attention: q {tuple(q.shape)} against prefix {tuple(prefix_k.shape)}: heads must "
+                         "be a multiple of the key / value heads, rows a multiple of the groups")
+    for t, m, what in ((lengths, B, "lengths"), (prefix_lengths, G, "prefix_lengths")):
+        if t is not None and (t.shape != (m,) or t.dtype not in (torch.int32, torch.int64) or t.device != q.device):
+            raise ValueError(f"shared_prefix_attention: {what} must be int32 or int64 [{m}] on {q.device}")
+    scale = D ** -0.5 if scale is None else float(scale)
+    if native_on(q) and q.dtype in (torch.bfloat16, torch.float16) and D in (64, 128) and Hq // Hk <= 128:
+        lengths, prefix_lengths = (t if t is None else t.contiguous() for t in (lengths, prefix_lengths))
+        return _C().shared_prefix_attention(_vec16(q), *(_vec16(t) for t in kv), lengths, prefix_lengths, scale)
+    return ref.shared_prefix_attention(q, *kv, lengths, prefix_lengths, scale)
+
+
+# ----------------------------------------------------------------------------------------------------------------------
+# sampling
+
+
+def sample(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,
+           return_logprob: bool = False):
+    """One token for each row of ``logits`` [..., V] (bf16, fp16 or fp32) from one uniform number a row, ``u`` [...]
+    (fp32, in [0, 1)).
+
+    The candidates are the logits that are neither -inf nor NaN, with weights exp((x - max) / temperature). In
+    descending order of x, ties by lowest index, they are cut to the first ``top_k`` (<= 0: all), then to the shortest
+    prefix that holds ``top_p`` of the weight left (>= 1: all), then to the weights of at least ``min_p`` (of the
+    largest, which is always kept). The token is the first kept index, in index order, whose running weight is greater
+    than u times the kept weight. temperature <= 0 (or NaN): the largest logit, lowest index first. Several logits of
+    +inf share the weight equally. A row without candidates gives token -1 and log-probability -inf.
+
+    Each of temperature, top_k, top_p and min_p is a number for all rows or a tensor [...] of one for each row (fp32;
+    top_k int32 or int64) on the logits' device; numbers are used as fp32. Returns int64 tokens [...], and with
+    ``return_logprob`` also the fp32 log-probability of each token under the distribution it was drawn from. Weights
+    and their sums are held in 64 bits, so tokens do not depend on how the work is divided."""
+    _no_grad_op("sample", logits)
+    if logits.dim() < 1 or logits.shape[-1] < 1:
+        raise ValueError(f"sample: logits {tuple(logits.shape)} must be [..., V] with at least one token")
+    if logits.dtype not in (torch.bfloat16, torch.float16, torch.float32):
+        raise ValueError(f"sample: logits must be bf16, fp16 or fp32, not {logits.dtype}")
+    lead, V = logits.shape[:-1], logits.shape[-1]
+    if u.shape != lead or u.dtype != torch.float32 or u.device != logits.device:
+        raise ValueError(f"sample: u must be fp32 {tuple(lead)} on {logits.device}")
+    pars = []
+    for name, x, lo, hi in (("temperature", temperature, 0.0, math.inf), ("top_k", top_k, -math.inf, math.inf),
+                            ("top_p", top_p, 0.0, math.inf), ("min_p", min_p, 0.0, 1.0)):
+        if isinstance(x, torch.Tensor):
+            types = (torch.int32, torch.int64) if name == "top_k" else (torch.float32,)
+            if x.shape != lead or x.dtype not in types or x.device != logits.device:
+                raise ValueError(f"sample: {name} must be a number or {types[0]} {tuple(lead)} on {logits.device}")
+            pars.append((x.reshape(-1).contiguous(), 0))
+            continue
+        if not lo <= x <= hi:
+            raise ValueError(f"sample: {name} = {x} is outside [{lo}, {hi}]")
+        pars.append((None, min(max(int(x), 0), V) if name == "top_k" else float(x)))
+    rows = logits if logits.dim() == 2 else logits.reshape(-1, V)
+    uu = u.reshape(-1).contiguous()
+    if native_on(logits):
+        rows = rows if rows.stride(1) == 1 or V == 1 else rows.contiguous()
+        tok, lp = _C().sample(rows, uu, *(y for x in pars for y in x), bool(return_logprob))
+    else:
+        full = [t if t is not None else torch.full((rows.shape[0],), x, device=rows.device,
+                                                   dtype=torch.int64 if i == 1 else torch.float32)
+                for i, (t, x) in enumerate(pars)]
+        tok, lp = ref.sample(rows, uu, *full)
+    if logits.dim() != 2:
+        tok, lp = tok.view(lead), (lp.view(lead) if return_logprob else None)
+    return (tok, lp) if return_logprob else tok
+
+
 # ----------------------------------------------------------------------------------------------------------------------
 # token embedding (x scale)
 
@@ -564,7 +674,7 @@ class _NativeEmbedding(torch.autograd.Function):
 def embedding(tokens: torch.Tensor, w: torch.Tensor, scale: float) -> torch.Tensor:
     if native_on(w):
         shp = tokens.shape
-        return _NativeEmbedding.apply(tokens.reshape(-1), w, scale).view(*shp, w.shape[1])
+        return _NativeEmbedding.apply(tokens.reshape(-1).contiguous(), w, scale).view(*shp, w.shape[1])
     return scale * F.embedding(tokens, w)
 
 
@@ -599,5 +709,6 @@ def cross_entropy(logits: torch.Tensor, target: torch.Tensor, ignore_index: int)
 
 __all__ = [
     "set_backend", "get_backend", "gemm", "linear", "rms_norm", "swiglu", "rope", "subln_swiglu", "gate_logsigmoid",
-    "retention", "retention_prefill", "retention_decode", "attention", "embedding", "cross_entropy", "ref",
+    "retention", "retention_prefill", "retention_decode", "attention", "shared_prefix_attention", "sample",
+    "embedding", "cross_entropy", "ref",
 ]

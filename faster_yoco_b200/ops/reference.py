@@ -227,6 +227,83 @@ def attention(q, k, v, causal: bool = True, window: Optional[int] = None, q_offs
     return o.transpose(1, 2).to(q.dtype)
 
 
+def shared_prefix_attention(q, prefix_k, prefix_v, k, v, lengths=None, prefix_lengths=None,
+                            softmax_scale: Optional[float] = None):
+    """q: [B,Lq,Hq,D]; prefix_k / prefix_v: [G,P,Hk,D], shared by the B // G consecutive rows of each group;
+    k / v: [B,S,Hk,D], the rows' own positions. Query i of row b sees prefix keys j < prefix_lengths[g] (default P) and
+    own keys j <= lengths[b] - Lq + i, j < lengths[b] (default S; both clamped to what is stored). fp32 math; a
+    query that sees no key gets zeros. Values behind the lengths are not read into the sums, whatever they hold."""
+    B, Lq, Hq, D = q.shape
+    G, P, Hk = prefix_k.shape[:3]
+    S, n, rep, dev = k.shape[1], B // max(G, 1), Hq // Hk, q.device
+    scale = softmax_scale if softmax_scale is not None else D ** -0.5
+    wide = torch.float64 if q.dtype == torch.float64 else torch.float32
+    full = lambda m, x: torch.full((m,), x, dtype=torch.long, device=dev)
+    own = full(B, S) if lengths is None else lengths.long().clamp(0, S)
+    pre = full(G, P) if prefix_lengths is None else prefix_lengths.long().clamp(0, P)
+    own_used = torch.arange(S, device=dev) < own[:, None]                                      # [B, S]
+    pre_used = torch.arange(P, device=dev) < pre[:, None]                                      # [G, P]
+    last = own[:, None] - Lq + torch.arange(Lq, device=dev)                                    # [B, Lq]
+    sees = own_used[:, None] & (torch.arange(S, device=dev) <= last[..., None])                # [B, Lq, S]
+    clean = lambda t, used: t.to(wide).masked_fill(~used[:, :, None, None], 0).transpose(1, 2)  # [.., Hk, keys, D]
+    pk, pv = clean(prefix_k, pre_used), clean(prefix_v, pre_used)
+    ok, ov = clean(k, own_used), clean(v, own_used)
+    qf = (q.to(wide) * scale).view(B, Lq, Hk, rep, D).permute(0, 2, 1, 3, 4)                   # [B, Hk, Lq, rep, D]
+    fold = lambda t, w: t.reshape(G, n, Hk, Lq * rep, w).transpose(1, 2).reshape(G, Hk, n * Lq * rep, w)
+    unfold = lambda t, w: t.reshape(G, Hk, n, Lq * rep, w).transpose(1, 2).reshape(B, Hk, Lq, rep, w)
+    if B == 0 or Lq == 0:
+        return torch.empty_like(q)
+    s0 = unfold((fold(qf, D) @ pk.transpose(-1, -2)).masked_fill(~pre_used[:, None, None], float("-inf")), P)
+    s1 = torch.einsum("bhird,bhjd->bhirj", qf, ok).masked_fill(~sees[:, None, :, None], float("-inf"))
+    s = torch.cat([s0, s1], -1)
+    if P + S == 0:
+        return torch.zeros_like(q)
+    top = s.amax(-1, keepdim=True)
+    w = torch.exp(s - top.masked_fill(top == float("-inf"), 0))
+    o = unfold(fold(w[..., :P], P) @ pv, D) + torch.einsum("bhirj,bhjd->bhird", w[..., P:], ov)
+    total = w.sum(-1, keepdim=True)
+    o = torch.where(total > 0, o / total, torch.zeros_like(o))
+    return o.permute(0, 2, 1, 3, 4).reshape(B, Lq, Hq, D).to(q.dtype)
+
+
+# ----------------------------------------------------------------------------------------------------------------------
+# sampling
+
+
+def sample(logits: torch.Tensor, u: torch.Tensor, temperature: torch.Tensor, top_k: torch.Tensor,
+           top_p: torch.Tensor, min_p: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """logits [N, V]; u, temperature, top_k, top_p, min_p: [N]. (token int64 [N], log-probability fp32 [N]).
+
+    Weights exp((x - max) / temperature) in 64 bits over the logits that are neither -inf nor NaN; in descending order
+    (ties: lowest index first) the first top_k are kept (<= 0: all), of those the shortest prefix with at least top_p of
+    their weight (>= 1: all), of those the weights >= min_p; the largest is always kept. The token is the first kept
+    index, in index order, whose running weight passes u times the kept weight. temperature <= 0: the largest logit.
+    Nothing to draw from: token -1, log-probability -inf."""
+    N, V = logits.shape
+    x = torch.where(torch.isnan(logits), float("-inf"), logits.double())
+    val, order = torch.sort(x, dim=-1, descending=True, stable=True)
+    top = val[:, :1]
+    t = temperature.double()[:, None]
+    rank = torch.arange(V, device=x.device).expand(N, V)
+    w = torch.exp(torch.where(val == top, 0.0, val - top) / torch.where(t > 0, t, 1.0))
+    w = torch.where(t > 0, w, (rank == 0).double()).masked_fill(val == float("-inf"), 0.0)
+    k = top_k.long()[:, None]
+    w = torch.where((rank < k) | (k <= 0), w, 0.0)
+    run = w.cumsum(-1)
+    before = F.pad(run, (1, 0))[:, :-1]
+    p = top_p.double()[:, None]
+    keep = (before < p * run[:, -1:]) | (p >= 1)
+    keep = (keep & (w >= min_p.double()[:, None])) | (rank == 0)
+    w = torch.zeros_like(w).scatter(1, order, torch.where(keep, w, 0.0))
+    run = w.cumsum(-1)
+    total = run[:, -1:]
+    pick = (run <= u.double()[:, None] * total).sum(-1, keepdim=True)
+    pick = torch.minimum(pick, torch.where(w > 0, rank, 0).amax(-1, keepdim=True))
+    lp = torch.log(w.gather(1, pick) / total).squeeze(1).float()
+    none = top.squeeze(1) == float("-inf")
+    return pick.squeeze(1).masked_fill(none, -1), lp.masked_fill(none, float("-inf"))
+
+
 # ----------------------------------------------------------------------------------------------------------------------
 # loss / optimizer
 
