@@ -1,5 +1,28 @@
-// Decode attention of a batch whose rows share long prefixes: query i of row b sees the prefix keys of its group and its
-// row's own keys up to its position.
+// Decode attention of a batch whose rows share long prefixes that are stored, and read, once (sm_100a, tcgen05).
+//
+// Query i of row b sees the prefix keys of its group and its row's own keys up to its position:
+//   o = sum_j e^(s_j - m) v_j / sum_j e^(s_j - m),   s_j = scale q . k_j
+// The sum splits over the keys: each piece gives (m, l = sum e^(s - m), O = sum e^(s - m) v) and pieces join by weights
+// e^(m - max m). All queries of a group against one key / value head (rows x queries x heads of the GQA group) are the
+// rows of ONE matrix product over the prefix, so its keys and values are read once for all of them; the own keys of each
+// row are a second, smaller product.
+//
+// Two kernels. spa_kernel, one persistent CTA an SM, walks 128-key tiles; spa_join_kernel joins the pieces, a warp for
+// each output row. The tiles of all (group, head, 128-row block) are one line that is cut into equal ranges, so every SM
+// has the same number of tiles whatever the number of heads, and a piece is the part of one block's tiles that falls
+// into one range. Lengths are read on the device: ranges are cut from the stored sizes, tiles behind a length are
+// skipped.
+//
+// Inside a CTA two streams of tiles run side by side, each with its own query block, scores S and output O in tensor
+// memory; one stream's softmax overlaps the other's products:
+//   warp 0      loads K / V tiles by TMA into a two-slot ring that both streams share
+//   warp 1      issues S = Q K^T and O += P V (P, rounded to the inputs' type, over the first columns of S)
+//   warp 2      copies the query block of the next piece into shared memory (rows of any stride)
+//   warps 3-6, 7-10   softmax of stream 0 / 1, a thread a query row: running maximum (O is rescaled only when it grows
+//               by more than 2^8), exponentials, row sums in fp32, P back to tensor memory; at the end of a piece O, m, l
+//               to the workspace
+// Work comes in three classes: (0) prefix blocks in pairs, both streams on the same K / V tile (compute bound: halves
+// the shared memory fills); (1) the odd last prefix block, each stream with tiles of its own; (2) own keys.
 #include <ATen/ATen.h>
 #include <c10/util/Optional.h>
 #include <cuda_fp16.h>
@@ -10,19 +33,37 @@
 namespace fyb {
 namespace {
 
-struct View {               // [rows, keys, heads, D], last dim contiguous
+constexpr int kT = 128;                 // tile: keys, and query rows
+constexpr int kBox = 32;                // key rows of one TMA box: what a tile's tail is rounded up to
+constexpr int kAtom = kT * 128;         // 128 rows of a 128-byte swizzle atom
+constexpr int kSpaThreads = 352;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kRescaleLog2 = 8.0f;
+
+struct View {                           // [rows, keys, heads, D], last dim contiguous
   const void* p;
   int64_t s0, s1, s2;
 };
 
 struct PrefixParams {
-  View q, pk, pv, k, v;
+  View q;
   int B, Lq, Hq, Hk, G, P, S;
-  const void* lengths;      // per row (int32 or int64), or null: S
+  int rep, rows_p, rows_o;              // heads of a GQA group; query rows of (group, head), of (row, head)
+  int pairs, odd, own_blocks;           // 128-row blocks: pairs and 0 / 1 more for the prefix, blocks of own keys
+  int tiles_p, tiles_o;                 // stored tiles
+  int64_t total[3];                     // tiles of each class
+  int units[3];                         // ranges that each class is cut into, none of them empty
+  int shift;                            // first stream that takes a range of class 2
+  int ctas;
+  const void* lengths;                  // per row (int32 or int64), or null: S
   const void* prefix_lengths;
   int lengths_64, prefix_lengths_64;
-  float scale;
-  void* o;                  // [B, Lq, Hq, D] contiguous
+  float scale_log2;
+  void* o;                              // [B, Lq, Hq, D] contiguous
+  float* part[3];                       // pieces: [slot][rows of the class][D]
+  float2* stat[3];                      // (m in log2 units, l) of each row
+  int part_rows[3];
+  int* status;
 };
 
 __device__ __forceinline__ int length_of(const void* p, int wide, int i, int most) {
@@ -31,52 +72,532 @@ __device__ __forceinline__ int length_of(const void* p, int wide, int i, int mos
   return static_cast<int>(n < 0 ? 0 : (n > most ? most : n));
 }
 
-__device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
-__device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
 template <typename T>
-__device__ __forceinline__ T from_float(float x);
+__device__ __forceinline__ uint32_t pack2(float lo, float hi);
 template <>
-__device__ __forceinline__ __half from_float<__half>(float x) { return __float2half_rn(x); }
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) { return pack_bf16(lo, hi); }
 template <>
-__device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+__device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
+  __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<uint32_t*>(&v);
+}
 
-// one warp for each (row, query, head), one key at a time with the running maximum and sum
+// instruction descriptor of kind::f16 with fp32 accumulation; the format bits are 1 for bf16 and 0 for fp16
+template <typename T>
+__device__ __forceinline__ constexpr uint32_t idesc_of(int N, bool b_mn) {
+  const uint32_t d = idesc_bf16(128, N, false, b_mn);
+  return sizeof(T) == 2 && !std::is_same<T, __nv_bfloat16>::value ? d & ~((7u << 7) | (7u << 10)) : d;
+}
+
+// K-major operand of 64-wide atoms; MN-major operand whose atoms are kAtom apart
+__device__ __forceinline__ uint64_t desc_k(uint32_t base, int k16) {
+  return sw128_desc(base + (k16 >> 2) * kAtom + (k16 & 3) * 32, 16, 1024);
+}
+__device__ __forceinline__ uint64_t desc_mn(uint32_t base, int k16) {
+  return sw128_desc(base + k16 * 2048, kAtom, 1024);
+}
+
+// range w of n takes tiles [w total / n, (w + 1) total / n); n <= total, so that no range is empty
+__device__ __forceinline__ int64_t range_begin(int64_t w, int64_t total, int64_t n) { return w * total / n; }
+__device__ __forceinline__ int64_t range_of(int64_t tile, int64_t total, int64_t n) {
+  return ((tile + 1) * n - 1) / total;
+}
+
+// The pieces of one stream in order; every role walks its own copy.
+struct Walk {
+  int cls = -1;
+  int64_t pos = 0, end = 0;
+  int seg = 0, t = 0, t1 = 0;     // current piece: tiles t .. t1 of block seg
+  int row = 0, hk = 0, blk = 0;   // group (classes 0, 1) or batch row (2), key / value head, 128-row block
+  int len = 0;                    // keys in use
+  int range = 0;
+
+  __device__ __forceinline__ bool next_piece(const PrefixParams& p, int cta, int stream) {
+    for (;;) {
+      while (pos >= end) {
+        if (++cls > 2) return false;
+        // class 0: a range a CTA; else a range a stream, first all CTAs' first streams, so that few ranges spread
+        // over the machine; class 2 starts behind the streams that class 1 gave work to
+        range = cls == 0 ? cta : stream * p.ctas + cta;
+        if (cls == 2) range = range >= p.shift ? range - p.shift : range - p.shift + 2 * p.ctas;
+        if (range < p.units[cls]) {
+          pos = range_begin(range, p.total[cls], p.units[cls]);
+          end = range_begin(range + 1, p.total[cls], p.units[cls]);
+        }
+      }
+      const int tiles = cls == 2 ? p.tiles_o : p.tiles_p;
+      seg = static_cast<int>(pos / tiles);
+      t = static_cast<int>(pos - static_cast<int64_t>(seg) * tiles);
+      const int64_t left = end - pos;
+      const int take = tiles - t < left ? tiles - t : static_cast<int>(left);
+      pos += take;
+      const int per = cls == 0 ? p.pairs : (cls == 1 ? 1 : p.own_blocks);
+      const int x = seg / per;
+      hk = x % p.Hk;
+      row = x / p.Hk;
+      blk = cls == 0 ? 2 * (seg % per) + stream : (cls == 1 ? 2 * p.pairs : seg % per);
+      len = cls == 2 ? length_of(p.lengths, p.lengths_64, row, p.S)
+                     : length_of(p.prefix_lengths, p.prefix_lengths_64, row, p.P);
+      t1 = min(t + take, (len + kT - 1) / kT);
+      if (t < t1) return true;
+    }
+  }
+  __device__ __forceinline__ int rows(const PrefixParams& p) const {
+    return min(kT, (cls == 2 ? p.rows_o : p.rows_p) - blk * kT);
+  }
+  // batch row, query and query head of row r of the block
+  __device__ __forceinline__ void locate(const PrefixParams& p, int r, int& b, int& i, int& h) const {
+    const int flat = blk * kT + r, tok = flat / p.rep;
+    h = hk * p.rep + flat - tok * p.rep;
+    const int bi = cls == 2 ? 0 : tok / p.Lq;
+    i = tok - bi * p.Lq;
+    b = cls == 2 ? row : row * (p.B / p.G) + bi;
+  }
+};
+
+template <typename V>
+__device__ __forceinline__ void exchange(V& a, V& b) {
+  V c = a;
+  a = b;
+  b = c;
+}
+
+// The tiles of a CTA in the order in which they are loaded and multiplied: the two streams in turn, each with a role's
+// state. The streams change places rather than being indexed, which keeps them in registers.
+template <typename State>
+struct Steps {
+  Walk w, w_other;
+  State s, s_other;                // of the stream whose turn it is, of the other one
+  bool live, live_other;
+  int turn = 0;                    // stream of the next step
+
+  __device__ __forceinline__ void start(const PrefixParams& p, int cta) {
+    live = w.next_piece(p, cta, 0);
+    live_other = w_other.next_piece(p, cta, 1);
+    if (!live && live_other) swap();
+  }
+  __device__ __forceinline__ void swap() {
+    exchange(w, w_other);
+    exchange(s, s_other);
+    exchange(live, live_other);
+    turn ^= 1;
+  }
+  // after a step: the stream's next tile, and the other stream's turn if it has one
+  __device__ __forceinline__ void advance(const PrefixParams& p, int cta) {
+    if (++w.t >= w.t1) live = w.next_piece(p, cta, turn);
+    if (live_other) swap();
+  }
+  // in class 0 stream 1 multiplies by the tile that stream 0 had loaded
+  __device__ __forceinline__ bool follows() const { return w.cls == 0 && turn == 1; }
+};
+struct Stateless {};
+
+struct SpaBars {
+  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];
+  uint64_t q_full[2], q_empty[2], s_full[2], p_full[2], o_full[2];   // by stream
+};
+
+template <int D>
+constexpr int spa_smem() {
+  return 6 * kT * D * 2 + 256 + 1024;
+}
+
 template <typename T, int D>
-__global__ void shared_prefix_kernel(PrefixParams p) {
+__global__ void __launch_bounds__(kSpaThreads, 1)
+    spa_kernel(const __grid_constant__ CUtensorMap tm_pk, const __grid_constant__ CUtensorMap tm_pv,
+               const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
+               const __grid_constant__ PrefixParams p) {
+  constexpr int kTile = kT * D * 2;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sQ = smem;                       // one block a stream
+  uint8_t* sK = sQ + 2 * kTile;             // ring
+  uint8_t* sV = sK + 2 * kTile;
+  SpaBars* bars = reinterpret_cast<SpaBars*>(sV + 2 * kTile);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int cta = blockIdx.x;
+  if (threadIdx.x == 0) {
+    uint64_t* all = reinterpret_cast<uint64_t*>(bars);
+    for (int i = 0; i < static_cast<int>(sizeof(SpaBars) / 8); ++i) mbar_init(&all[i], 1);
+    for (int s = 0; s < 2; ++s) mbar_init(&bars->p_full[s], 4);
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;         // S of stream s (P over its first columns) @ 128 s, O @ 256 + 128 s
+
+  if (warp == 0) {
+    // ------------------------------------------------------------------------------------------------ K / V loads
+    if (lane == 0) {
+      Steps<Stateless> st;
+      st.start(p, cta);
+      int nk = 0, nv = 0;
+      for (; st.live; st.advance(p, cta)) {
+        if (st.follows()) continue;
+        const Walk& x = st.w;
+        const int slot = nk & 1;
+        const uint32_t ph = ((nk >> 1) & 1) ^ 1u;
+        const int boxes = (min(kT, x.len - x.t * kT) + kBox - 1) / kBox;
+        const uint32_t bytes = boxes * kBox * D * 2;
+        auto load = [&](uint8_t* dst, const CUtensorMap* m, uint64_t* bar) {
+          mbar_arrive_expect_tx(bar, bytes);
+          for (int j = 0; j < boxes; ++j)
+#pragma unroll
+            for (int a = 0; a < D / 64; ++a)
+              tma_load_4d(dst + a * kAtom + j * kBox * 128, m, bar, a * 64, x.hk, x.t * kT + j * kBox, x.row);
+        };
+        if (!mbar_wait(&bars->k_empty[slot], ph, abort_flag, p.status, 700)) break;
+        load(sK + slot * kTile, x.cls == 2 ? &tm_k : &tm_pk, &bars->k_full[slot]);
+        ++nk;
+        if (!mbar_wait(&bars->v_empty[slot], ph, abort_flag, p.status, 701)) break;
+        load(sV + slot * kTile, x.cls == 2 ? &tm_v : &tm_pv, &bars->v_full[slot]);
+        ++nv;
+      }
+      // before the CTA ends its loads have landed, and without a timeout have been read
+      for (int i = max(nk - 2, 0); i < nk; ++i) mbar_wait(&bars->k_full[i & 1], (i >> 1) & 1, nullptr, p.status, 702);
+      for (int i = max(nv - 2, 0); i < nv; ++i) mbar_wait(&bars->v_full[i & 1], (i >> 1) & 1, nullptr, p.status, 703);
+      for (int i = max(nk - 2, 0); i < nk && !*abort_flag; ++i)
+        mbar_wait(&bars->k_empty[i & 1], (i >> 1) & 1, abort_flag, p.status, 704);
+      for (int i = max(nv - 2, 0); i < nv && !*abort_flag; ++i)
+        mbar_wait(&bars->v_empty[i & 1], (i >> 1) & 1, abort_flag, p.status, 705);
+    }
+  } else if (warp == 1) {
+    // --------------------------------------------------------------------------------------------- matrix products
+    struct Product {
+      bool pending = false, first = true;    // P V of the stream's last tile is still to be issued; a piece starts
+      bool opens, last, frees, fix;          // of that product: first / last of its piece, last reader of its V tile
+      int slot, nv;
+      uint32_t vph, pph = 0, qph = 0;
+    };
+    Steps<Product> st;
+    st.start(p, cta);
+    int n = 0;                               // loads met so far
+    bool ok = true;
+    auto wait = [&](uint64_t* bar, uint32_t ph, int site) -> bool {
+      int good = 1;
+      if (lane == 0) good = mbar_wait(bar, ph, abort_flag, p.status, site) ? 1 : 0;
+      good = __shfl_sync(0xffffffffu, good, 0);
+      __syncwarp();
+      return good != 0;
+    };
+    auto issue_pv = [&](Product& v, int s) -> bool {
+      v.pending = false;
+      if (!wait(&bars->p_full[s], v.pph, 710)) return false;
+      v.pph ^= 1u;
+      if (!wait(&bars->v_full[v.slot], v.vph, 711)) return false;
+      uint8_t* tile = sV + v.slot * kTile;
+      const int steps = (v.nv + 15) / 16;
+      if (v.fix && v.nv < steps * 16) {
+        // a weight of zero times what lies behind the last key in use has to be zero (whole rows: no swizzle)
+        for (int c = lane; c < (steps * 16 - v.nv) * (D / 8); c += 32) {
+          const int r = v.nv + c / (D / 8), ch = c % (D / 8);
+          *reinterpret_cast<uint4*>(tile + (ch >> 3) * kAtom + r * 128 + (ch & 7) * 16) = make_uint4(0, 0, 0, 0);
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+      }
+      if (lane == 0) {
+        tc_fence_after();
+        const uint32_t a = smem_u32(tile);
+        for (int k = 0; k < steps; ++k)
+          umma_bf16_ts(tmem + 256 + 128 * s, tmem + 128 * s + k * 8, desc_mn(a, k), idesc_of<T>(D, true),
+                       (v.opens && k == 0) ? 0u : 1u);
+        if (v.frees) umma_commit(&bars->v_empty[v.slot]);
+        if (v.last) umma_commit(&bars->o_full[s]);
+      }
+      __syncwarp();
+      return true;
+    };
+    for (; ok && st.live; st.advance(p, cta)) {
+      const int s = st.turn;
+      const Walk& x = st.w;
+      if (st.s.pending && !(ok = issue_pv(st.s, s))) break;
+      // a stream that has ended must not hold its V tile while the other goes on (its product is the younger one)
+      if (!st.live_other && st.s_other.pending && !(ok = issue_pv(st.s_other, s ^ 1))) break;
+      const bool follows = st.follows();
+      const int ring = follows ? n - 1 : n;
+      const int slot = ring & 1;
+      const uint32_t ph = (ring >> 1) & 1;
+      const int nv = min(kT, x.len - x.t * kT);
+      const bool last = x.t + 1 >= x.t1, frees = x.cls != 0 || follows;
+      if (!follows) {
+        if (!(ok = wait(&bars->k_full[slot], ph, 712))) break;
+        ++n;
+      }
+      if (st.s.first) {
+        if (!(ok = wait(&bars->q_full[s], st.s.qph, 713))) break;
+        st.s.qph ^= 1u;
+      }
+      if (lane == 0) {
+        tc_fence_after();
+        const uint32_t aq = smem_u32(sQ + s * kTile), ak = smem_u32(sK + slot * kTile);
+        const uint32_t id = idesc_of<T>((nv + 15) / 16 * 16, false);
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) umma_bf16(tmem + 128 * s, desc_k(aq, k), desc_k(ak, k), id, k > 0 ? 1u : 0u);
+        umma_commit(&bars->s_full[s]);
+        if (frees) umma_commit(&bars->k_empty[slot]);
+        if (last) umma_commit(&bars->q_empty[s]);
+      }
+      __syncwarp();
+      st.s.pending = true;
+      st.s.opens = st.s.first;
+      st.s.last = last;
+      st.s.frees = frees;
+      st.s.fix = !follows;
+      st.s.slot = slot;
+      st.s.nv = nv;
+      st.s.vph = ph;
+      st.s.first = last;
+    }
+    // the products left over: the stream that did not take the last step holds the older one
+    if (ok && st.s_other.pending) ok = issue_pv(st.s_other, st.turn ^ 1);
+    if (ok && st.s.pending) ok = issue_pv(st.s, st.turn);
+  } else if (warp == 2) {
+    // ----------------------------------------------------------------------------------------------- query blocks
+    struct Pieces {
+      bool first = true;
+      int n = 0;
+    };
+    Steps<Pieces> st;
+    st.start(p, cta);
+    bool ok = true;
+    for (; st.live; st.advance(p, cta)) {
+      const int s = st.turn;
+      const Walk& x = st.w;
+      if (st.s.first) {
+        int good = 1;
+        if (lane == 0) good = mbar_wait(&bars->q_empty[s], (st.s.n & 1) ^ 1u, abort_flag, p.status, 720) ? 1 : 0;
+        if (!(ok = __shfl_sync(0xffffffffu, good, 0) != 0)) break;
+        __syncwarp();
+        const int chunks = x.rows(p) * (D / 8);
+        for (int c = lane; c < chunks; c += 32) {
+          const int r = c / (D / 8), ch = c % (D / 8);
+          int b, i, h;
+          x.locate(p, r, b, i, h);
+          const T* src = reinterpret_cast<const T*>(p.q.p) + b * p.q.s0 + i * p.q.s1 + h * p.q.s2 + ch * 8;
+          cp_async16(sQ + s * kTile + (ch >> 3) * kAtom + r * 128 + (((ch & 7) ^ (r & 7)) << 4), src);
+        }
+        cp_async_wait_all();
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars->q_full[s]);
+        ++st.s.n;
+      }
+      st.s.first = x.t + 1 >= x.t1;
+    }
+    if (ok && lane == 0) {
+      if (st.s.n > 0) mbar_wait(&bars->q_empty[st.turn], (st.s.n - 1) & 1, abort_flag, p.status, 721);
+      if (st.s_other.n > 0)
+        mbar_wait(&bars->q_empty[st.turn ^ 1], (st.s_other.n - 1) & 1, abort_flag, p.status, 722);
+    }
+  } else {
+    // ---------------------------------------------------------------------------------------------------- softmax
+    const int s = warp >= 7 ? 1 : 0;
+    const int quad = warp & 3;
+    const int r = quad * 32 + lane;
+    const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
+    const uint32_t tS = tmem + 128 * s + lanes, tO = tmem + 256 + 128 * s + lanes;
+    // fp16 weights are lifted by 2^7 (at most 2^15 with the lazy maximum), which keeps what lies down to 2^-21 of the
+    // largest in its normal range; bf16 has fp32's range
+    constexpr float kLift = std::is_same<T, __half>::value ? 7.0f : 0.0f;
+    Walk x;
+    uint32_t s_ph = 0, o_ph = 0;
+    bool ok = true;
+    while (ok && x.next_piece(p, cta, s)) {
+      const int rows = x.rows(p);
+      const bool active = quad * 32 < rows;              // this warp has rows
+      int b, i, h;
+      x.locate(p, min(r, rows - 1), b, i, h);
+      // keys that this row sees: all in use of a prefix, of its own those up to its position
+      const int sees = x.cls == 2 ? min(x.len, x.len - p.Lq + i + 1) : x.len;
+      float m_ref = -INFINITY, l = 0.f;
+      for (; x.t < x.t1; ++x.t) {
+        if (!(ok = mbar_wait(&bars->s_full[s], s_ph, abort_flag, p.status, 730))) break;
+        s_ph ^= 1u;
+        if (active) {
+          tc_fence_after();
+          const int nv = min(kT, x.len - x.t * kT), vis = sees - x.t * kT;
+          uint32_t v[4][32];
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            if (c * 32 < nv) tmem_ld32(tS + c * 32, v[c]);
+          tmem_ld_wait();
+          float mx = -INFINITY;
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            if (c * 32 >= nv) continue;
+            if (vis < c * 32 + 32) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j)
+                if (c * 32 + j >= vis) v[c][j] = __float_as_uint(-INFINITY);
+            }
+#pragma unroll
+            for (int j = 0; j < 32; ++j) mx = fmaxf(mx, __uint_as_float(v[c][j]));
+          }
+          const float m_cand = fmaxf(m_ref, mx * p.scale_log2);
+          const bool need = m_cand > m_ref + kRescaleLog2;
+          const bool scale_o = need && m_ref != -INFINITY;
+          if (__any_sync(0xffffffffu, scale_o)) {
+            // the products up to the previous tile are complete: S, which this thread waited for, was issued after them
+            const float f = scale_o ? fast_exp2(m_ref - m_cand) : 1.0f;
+#pragma unroll
+            for (int c = 0; c < D; c += 16) {
+              uint32_t w[16];
+              tmem_ld16(tO + c, w);
+              tmem_ld_wait();
+#pragma unroll
+              for (int j = 0; j < 16; ++j) w[j] = __float_as_uint(__uint_as_float(w[j]) * f);
+              tmem_st16(tO + c, w);
+            }
+            if (scale_o) l *= f;
+          }
+          if (need) m_ref = m_cand;
+          const float m = m_ref == -INFINITY ? 0.f : m_ref - kLift;
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            if (c * 32 >= nv) continue;
+            uint32_t w[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              const float a = fast_exp2(__uint_as_float(v[c][2 * j]) * p.scale_log2 - m);
+              const float e = fast_exp2(__uint_as_float(v[c][2 * j + 1]) * p.scale_log2 - m);
+              l += a + e;
+              w[j] = pack2<T>(a, e);
+            }
+            tmem_st16(tS + c * 16, w);
+          }
+          tmem_st_wait();
+          tc_fence_before();
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars->p_full[s]);
+      }
+      if (!ok || !(ok = mbar_wait(&bars->o_full[s], o_ph, abort_flag, p.status, 731))) break;
+      o_ph ^= 1u;
+      if (active) {
+        tc_fence_after();
+        const int64_t slot = x.cls == 0 ? 2 * (static_cast<int64_t>(x.range) + x.seg) + s
+                                        : static_cast<int64_t>(x.range) + x.seg;
+        const int64_t at = slot * p.part_rows[x.cls] + r;
+        float* dst = p.part[x.cls] + at * D;
+#pragma unroll
+        for (int c = 0; c < D; c += 32) {
+          uint32_t v[32];
+          tmem_ld32(tO + c, v);
+          tmem_ld_wait();
+          if (r < rows) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              *reinterpret_cast<uint4*>(dst + c + 4 * j) = make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+          }
+        }
+        __syncwarp();
+        if (r < rows) p.stat[x.cls][at] = make_float2(m_ref - kLift, l);
+        tc_fence_before();
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// Joins the pieces of each output row (a warp a row): o = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i.
+template <typename T, int D>
+__global__ void __launch_bounds__(128) spa_join_kernel(const __grid_constant__ PrefixParams p) {
   constexpr int E = D / 32;
   const int64_t w = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
   const int lane = threadIdx.x & 31;
   if (w >= static_cast<int64_t>(p.B) * p.Lq * p.Hq) return;
   const int h = static_cast<int>(w % p.Hq);
-  const int i = static_cast<int>(w / p.Hq % p.Lq);
-  const int b = static_cast<int>(w / p.Hq / p.Lq);
-  const int hk = h / (p.Hq / p.Hk), g = b / (p.B / p.G);
-  float q[E], o[E];
-  const T* qp = reinterpret_cast<const T*>(p.q.p) + b * p.q.s0 + i * p.q.s1 + h * p.q.s2 + lane * E;
-  for (int e = 0; e < E; ++e) {
-    q[e] = to_float(qp[e]) * p.scale;
-    o[e] = 0.f;
-  }
-  float m = -INFINITY, l = 0.f;
-  auto walk = [&](const View& kk, const View& vv, int row, int n) {
-    for (int j = 0; j < n; ++j) {
-      const T* kp = reinterpret_cast<const T*>(kk.p) + row * kk.s0 + j * kk.s1 + hk * kk.s2 + lane * E;
-      float s = 0.f;
-      for (int e = 0; e < E; ++e) s += q[e] * to_float(kp[e]);
-      for (int x = 16; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-      const float mn = fmaxf(m, s);
-      const float f = m == -INFINITY ? 0.f : __expf(m - mn), a = __expf(s - mn);
-      m = mn;
-      l = l * f + a;
-      const T* vp = reinterpret_cast<const T*>(vv.p) + row * vv.s0 + j * vv.s1 + hk * vv.s2 + lane * E;
-      for (int e = 0; e < E; ++e) o[e] = o[e] * f + a * to_float(vp[e]);
+  const int64_t tok = w / p.Hq;
+  const int i = static_cast<int>(tok % p.Lq), b = static_cast<int>(tok / p.Lq);
+  const int hk = h / p.rep, n = p.B / p.G, g = b / n;
+
+  float M = -INFINITY, L = 0.f, o[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) o[e] = 0.f;
+  // pieces lo .. hi of class c: slot = mul * (range + seg) + add, row r of the slot
+  auto join = [&](int c, int seg, int tiles, int used, int mul, int add, int r) {
+    if (used == 0) return;
+    const int64_t t0 = static_cast<int64_t>(seg) * tiles;
+    const int lo = static_cast<int>(range_of(t0, p.total[c], p.units[c]));
+    const int hi = static_cast<int>(range_of(t0 + used - 1, p.total[c], p.units[c]));
+    for (int base = lo; base <= hi; base += 32) {
+      const int cnt = min(32, hi + 1 - base);
+      float2 ml = make_float2(-INFINITY, 0.f);
+      if (lane < cnt)
+        ml = p.stat[c][(mul * (static_cast<int64_t>(base) + lane + seg) + add) * p.part_rows[c] + r];
+      float mx = ml.y > 0.f ? ml.x : -INFINITY;
+#pragma unroll
+      for (int x = 16; x > 0; x >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+      if (mx == -INFINITY) continue;
+      const float Mn = fmaxf(M, mx);
+      const float f0 = M == -INFINITY ? 0.f : exp2f(M - Mn);
+      const float f = ml.y > 0.f ? exp2f(ml.x - Mn) : 0.f;
+      float lw = f * ml.y;
+#pragma unroll
+      for (int x = 16; x > 0; x >>= 1) lw += __shfl_xor_sync(0xffffffffu, lw, x);
+      L = L * f0 + lw;
+      M = Mn;
+#pragma unroll
+      for (int e = 0; e < E; ++e) o[e] *= f0;
+      for (int j = 0; j < cnt; ++j) {
+        const float fj = __shfl_sync(0xffffffffu, f, j);
+        const float* src =
+            p.part[c] + ((mul * (static_cast<int64_t>(base) + j + seg) + add) * p.part_rows[c] + r) * D + lane * E;
+        if constexpr (E == 4) {
+          const float4 t = *reinterpret_cast<const float4*>(src);
+          if (fj != 0.f) {
+            o[0] += fj * t.x;
+            o[1] += fj * t.y;
+            o[2] += fj * t.z;
+            o[3] += fj * t.w;
+          }
+        } else {
+          const float2 t = *reinterpret_cast<const float2*>(src);
+          if (fj != 0.f) {
+            o[0] += fj * t.x;
+            o[1] += fj * t.y;
+          }
+        }
+      }
     }
   };
-  walk(p.pk, p.pv, g, length_of(p.prefix_lengths, p.prefix_lengths_64, g, p.P));
-  const int own = length_of(p.lengths, p.lengths_64, b, p.S);
-  walk(p.k, p.v, b, max(0, own - p.Lq + i + 1));
+  {
+    const int flat = ((b - g * n) * p.Lq + i) * p.rep + h - hk * p.rep;
+    const int blk = flat / kT, r = flat - blk * kT, gh = g * p.Hk + hk;
+    const int used = (length_of(p.prefix_lengths, p.prefix_lengths_64, g, p.P) + kT - 1) / kT;
+    if (blk < 2 * p.pairs)
+      join(0, gh * p.pairs + (blk >> 1), p.tiles_p, used, 2, blk & 1, r);
+    else
+      join(1, gh, p.tiles_p, used, 1, 0, r);
+  }
+  {
+    const int flat = i * p.rep + h - hk * p.rep;
+    const int blk = flat / kT, r = flat - blk * kT;
+    const int used = (length_of(p.lengths, p.lengths_64, b, p.S) + kT - 1) / kT;
+    join(2, (b * p.Hk + hk) * p.own_blocks + blk, p.tiles_o, used, 1, 0, r);
+  }
+  const float inv = L > 0.f ? 1.0f / L : 0.f;
   T* op = reinterpret_cast<T*>(p.o) + w * D + lane * E;
-  for (int e = 0; e < E; ++e) op[e] = from_float<T>(l > 0.f ? o[e] / l : 0.f);
+  if constexpr (E == 4)
+    *reinterpret_cast<uint2*>(op) = make_uint2(pack2<T>(o[0] * inv, o[1] * inv), pack2<T>(o[2] * inv, o[3] * inv));
+  else
+    *reinterpret_cast<uint32_t*>(op) = pack2<T>(o[0] * inv, o[1] * inv);
 }
 
 View view_of(const at::Tensor& t, const at::Tensor& q, const char* name) {
@@ -91,6 +612,24 @@ View view_of(const at::Tensor& t, const at::Tensor& q, const char* name) {
   return View{t.data_ptr(), t.stride(0), t.stride(1), t.stride(2)};
 }
 
+// {D, heads, keys, rows} with boxes of 64 x 1 x kBox x 1; a dimension of one element has no stride to speak of
+CUtensorMap tmap_cache(const at::Tensor& t) {
+  if (t.numel() == 0) return CUtensorMap{};            // no tile of it is loaded
+  CUtensorMap m;
+  auto bytes = [&](int d) -> cuuint64_t { return t.size(d) > 1 ? t.stride(d) * 2 : t.size(3) * 2; };
+  cuuint64_t dims[4] = {(cuuint64_t)t.size(3), (cuuint64_t)t.size(2), (cuuint64_t)t.size(1), (cuuint64_t)t.size(0)};
+  cuuint64_t strides[3] = {bytes(2), bytes(1), bytes(0)};
+  cuuint32_t box[4] = {64u, 1u, (cuuint32_t)kBox, 1u};
+  cuuint32_t one[4] = {1u, 1u, 1u, 1u};
+  const CUresult r = encode_fn()(
+      &m, t.scalar_type() == at::kHalf ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
+      t.data_ptr(), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+      CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  FYB_CHECK(r == CUDA_SUCCESS,
+            "shared_prefix_attention: cuTensorMapEncodeTiled code " + std::to_string(static_cast<int>(r)));
+  return m;
+}
+
 const void* length_ptr(const c10::optional<at::Tensor>& t, const at::Tensor& q, int64_t n, int& wide) {
   wide = 0;
   if (!t.has_value() || !t->defined()) return nullptr;
@@ -99,6 +638,18 @@ const void* length_ptr(const c10::optional<at::Tensor>& t, const at::Tensor& q, 
                 (n <= 1 || t->stride(0) == 1),
             "shared_prefix_attention: lengths");
   return t->data_ptr();
+}
+
+template <typename T, int D>
+void launch(const CUtensorMap& pk, const CUtensorMap& pv, const CUtensorMap& k, const CUtensorMap& v,
+            const PrefixParams& p) {
+  // per call: the attribute belongs to the device that is current
+  FYB_CUDA(cudaFuncSetAttribute(spa_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, spa_smem<D>()));
+  spa_kernel<T, D><<<p.ctas, kSpaThreads, spa_smem<D>(), cur_stream()>>>(pk, pv, k, v, p);
+  check_launch("shared_prefix_attention");
+  const int64_t rows = (int64_t)p.B * p.Lq * p.Hq;
+  spa_join_kernel<T, D><<<(rows + 3) / 4, 128, 0, cur_stream()>>>(p);
+  check_launch("shared_prefix_attention (join)");
 }
 
 }  // namespace
@@ -111,33 +662,67 @@ at::Tensor shared_prefix_attention(const at::Tensor& q, const at::Tensor& pk, co
   FYB_CHECK(q.is_cuda() && q.dim() == 4 && (q.size(3) == 64 || q.size(3) == 128) &&
                 (q.scalar_type() == at::kBFloat16 || q.scalar_type() == at::kHalf),
             "shared_prefix_attention: bf16 or fp16 q [B, Lq, Hq, 64 or 128] expected");
+  FYB_CHECK(scale > 0 && std::isfinite(scale), "shared_prefix_attention: scale must be positive");
   const int64_t B = q.size(0), Lq = q.size(1), Hq = q.size(2), D = q.size(3);
   PrefixParams p{};
   p.q = view_of(q, q, "q");
-  p.pk = view_of(pk, q, "prefix_k");
-  p.pv = view_of(pv, q, "prefix_v");
-  p.k = view_of(k, q, "k");
-  p.v = view_of(v, q, "v");
+  view_of(pk, q, "prefix_k");
+  view_of(pv, q, "prefix_v");
+  view_of(k, q, "k");
+  view_of(v, q, "v");
   const int64_t G = pk.size(0), P = pk.size(1), Hk = pk.size(2), S = k.size(1);
   FYB_CHECK(pv.sizes() == pk.sizes() && v.sizes() == k.sizes() && k.size(0) == B && k.size(2) == Hk && Hk > 0 && G > 0 &&
-                Hq % Hk == 0 && Hq / Hk <= 128 && B % G == 0,
+                Hq > 0 && Hq % Hk == 0 && B % G == 0,
             "shared_prefix_attention: shape mismatch");
   FYB_CHECK(B * Lq * Hq < (1ll << 31) && P < (1ll << 30) && S < (1ll << 30), "shared_prefix_attention: sizes");
   c10::cuda::CUDAGuard guard(q.device());
   auto o = at::empty({B, Lq, Hq, D}, q.options());
   if (o.numel() == 0) return o;
   p.B = (int)B, p.Lq = (int)Lq, p.Hq = (int)Hq, p.Hk = (int)Hk, p.G = (int)G, p.P = (int)P, p.S = (int)S;
+  p.rep = (int)(Hq / Hk);
+  p.rows_p = (int)(B / G * Lq * p.rep);
+  p.rows_o = (int)(Lq * p.rep);
+  const int blocks = (p.rows_p + kT - 1) / kT;
+  p.pairs = blocks / 2;
+  p.odd = blocks & 1;
+  p.own_blocks = (p.rows_o + kT - 1) / kT;
+  p.tiles_p = (int)((P + kT - 1) / kT);
+  p.tiles_o = (int)((S + kT - 1) / kT);
+  const int64_t segs[3] = {G * Hk * p.pairs, G * Hk * p.odd, B * Hk * p.own_blocks};
+  for (int c = 0; c < 3; ++c) p.total[c] = segs[c] * (c == 2 ? p.tiles_o : p.tiles_p);
+  p.ctas = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
+  for (int c = 0; c < 3; ++c) p.units[c] = (int)std::min<int64_t>(p.total[c], c == 0 ? p.ctas : 2 * p.ctas);
+  p.shift = p.units[1] % (2 * p.ctas);
   p.lengths = length_ptr(lengths, q, B, p.lengths_64);
   p.prefix_lengths = length_ptr(prefix_lengths, q, G, p.prefix_lengths_64);
-  p.scale = (float)scale;
+  p.scale_log2 = (float)(scale * 1.4426950408889634);
   p.o = o.data_ptr();
-  const int64_t grid = (B * Lq * Hq + 3) / 4;
+  p.status = status_ptr();
+  // a slot for each (range, block) that can meet: ranges + blocks, as both only move forward
+  p.part_rows[0] = kT;
+  p.part_rows[1] = p.rows_p - 2 * p.pairs * kT;
+  p.part_rows[2] = std::min(p.rows_o, kT);
+  int64_t rows[3], all = 0;
+  for (int c = 0; c < 3; ++c) {
+    const int64_t slots = (p.units[c] + segs[c]) * (c == 0 ? 2 : 1);
+    rows[c] = p.total[c] > 0 ? slots * p.part_rows[c] : 0;
+    all += rows[c];
+  }
+  auto ws = at::empty({std::max<int64_t>(all, 1) * (D + 2)}, q.options().dtype(at::kFloat));
+  float* at_ = ws.data_ptr<float>();
+  for (int c = 0; c < 3; ++c) {
+    p.part[c] = at_;
+    at_ += rows[c] * D;
+  }
+  for (int c = 0; c < 3; ++c) {
+    p.stat[c] = reinterpret_cast<float2*>(at_);
+    at_ += rows[c] * 2;
+  }
+  const CUtensorMap mpk = tmap_cache(pk), mpv = tmap_cache(pv), mk = tmap_cache(k), mv = tmap_cache(v);
   if (q.scalar_type() == at::kBFloat16)
-    (D == 64 ? shared_prefix_kernel<__nv_bfloat16, 64> : shared_prefix_kernel<__nv_bfloat16, 128>)
-        <<<grid, 128, 0, cur_stream()>>>(p);
+    D == 64 ? launch<__nv_bfloat16, 64>(mpk, mpv, mk, mv, p) : launch<__nv_bfloat16, 128>(mpk, mpv, mk, mv, p);
   else
-    (D == 64 ? shared_prefix_kernel<__half, 64> : shared_prefix_kernel<__half, 128>)<<<grid, 128, 0, cur_stream()>>>(p);
-  check_launch("shared_prefix_attention");
+    D == 64 ? launch<__half, 64>(mpk, mpv, mk, mv, p) : launch<__half, 128>(mpk, mpv, mk, mv, p);
   return o;
 }
 

@@ -553,8 +553,7 @@ def shared_prefix_attention(q: torch.Tensor, prefix_k: torch.Tensor, prefix_v: t
     means all stored positions. Positions behind the lengths may hold anything. P, S, B or Lq may be 0; a query that
     sees no key gets zeros. scale: default 1 / sqrt(D). Returns a contiguous [B, Lq, Hq, D].
 
-    The sm_100a kernel takes bf16 and fp16 with D 64 or 128 and at most 128 query heads a key / value head; other
-    types and sizes run the PyTorch expression. Key / value tensors are read in place when their rows are 16-byte
+    The sm_100a kernel takes bf16 and fp16 with D 64 or 128; other types and sizes run the PyTorch expression. Key / value tensors are read in place when their rows are 16-byte
     aligned, else copied first. A value that SOME query of a row sees has to be finite. Inference only."""
     _no_grad_op("shared_prefix_attention", q, prefix_k, prefix_v, k, v)
     kv = (prefix_k, prefix_v, k, v)
@@ -574,7 +573,9 @@ def shared_prefix_attention(q: torch.Tensor, prefix_k: torch.Tensor, prefix_v: t
         if t is not None and (t.shape != (m,) or t.dtype not in (torch.int32, torch.int64) or t.device != q.device):
             raise ValueError(f"shared_prefix_attention: {what} must be int32 or int64 [{m}] on {q.device}")
     scale = D ** -0.5 if scale is None else float(scale)
-    if native_on(q) and q.dtype in (torch.bfloat16, torch.float16) and D in (64, 128) and Hq // Hk <= 128:
+    if not 0.0 < scale < math.inf:
+        raise ValueError(f"shared_prefix_attention: scale = {scale} must be positive and finite")
+    if native_on(q) and q.dtype in (torch.bfloat16, torch.float16) and D in (64, 128):
         lengths, prefix_lengths = (t if t is None else t.contiguous() for t in (lengths, prefix_lengths))
         return _C().shared_prefix_attention(_vec16(q), *(_vec16(t) for t in kv), lengths, prefix_lengths, scale)
     return ref.shared_prefix_attention(q, *kv, lengths, prefix_lengths, scale)
