@@ -15,10 +15,10 @@
 //
 // Inside a CTA two streams of tiles run side by side, each with its own query block, scores S and output O in tensor
 // memory; one stream's softmax overlaps the other's products:
-//   warp 0      loads K / V tiles by TMA into a two-slot ring that both streams share
+//   warp 0      loads K / V tiles by TMA, in the order in which they are multiplied, into one ring of slots
 //   warp 1      issues S = Q K^T and O += P V (P, rounded to the inputs' type, over the first columns of S)
-//   warp 2      copies the query block of the next piece into shared memory (rows of any stride)
-//   warps 3-6, 7-10   softmax of stream 0 / 1, a thread a query row: running maximum (O is rescaled only when it grows
+//   warps 2, 3  copy the query block of the next piece of stream 0 / 1 into shared memory (rows of any stride)
+//   warps 4-7, 8-11   softmax of stream 0 / 1, a thread a query row: running maximum (O is rescaled only when it grows
 //               by more than 2^8), exponentials, row sums in fp32, P back to tensor memory; at the end of a piece O, m, l
 //               to the workspace
 // Work comes in three classes: (0) prefix blocks in pairs, both streams on the same K / V tile (compute bound: halves
@@ -34,9 +34,10 @@ namespace fyb {
 namespace {
 
 constexpr int kT = 128;                 // tile: keys, and query rows
-constexpr int kBox = 32;                // key rows of one TMA box: what a tile's tail is rounded up to
+constexpr int kOwnBox = 32;             // key rows of one TMA box of own keys: what their last tile is rounded up to
 constexpr int kAtom = kT * 128;         // 128 rows of a 128-byte swizzle atom
-constexpr int kSpaThreads = 352;
+constexpr int kSpaThreads = 384;
+constexpr int kJoinWarps = 4;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRescaleLog2 = 8.0f;
 
@@ -51,7 +52,7 @@ struct PrefixParams {
   int rep, rows_p, rows_o;              // heads of a GQA group; query rows of (group, head), of (row, head)
   int pairs, odd, own_blocks;           // 128-row blocks: pairs and 0 / 1 more for the prefix, blocks of own keys
   int tiles_p, tiles_o;                 // stored tiles
-  int64_t total[3];                     // tiles of each class
+  int total[3];                         // tiles of each class
   int units[3];                         // ranges that each class is cut into, none of them empty
   int shift;                            // first stream that takes a range of class 2
   int ctas;
@@ -98,15 +99,15 @@ __device__ __forceinline__ uint64_t desc_mn(uint32_t base, int k16) {
 }
 
 // range w of n takes tiles [w total / n, (w + 1) total / n); n <= total, so that no range is empty
-__device__ __forceinline__ int64_t range_begin(int64_t w, int64_t total, int64_t n) { return w * total / n; }
-__device__ __forceinline__ int64_t range_of(int64_t tile, int64_t total, int64_t n) {
-  return ((tile + 1) * n - 1) / total;
+__device__ __forceinline__ int range_begin(int64_t w, int total, int n) { return static_cast<int>(w * total / n); }
+__device__ __forceinline__ int range_of(int64_t tile, int total, int n) {
+  return static_cast<int>(((tile + 1) * n - 1) / total);
 }
 
 // The pieces of one stream in order; every role walks its own copy.
 struct Walk {
   int cls = -1;
-  int64_t pos = 0, end = 0;
+  int pos = 0, end = 0;
   int seg = 0, t = 0, t1 = 0;     // current piece: tiles t .. t1 of block seg
   int row = 0, hk = 0, blk = 0;   // group (classes 0, 1) or batch row (2), key / value head, 128-row block
   int len = 0;                    // keys in use
@@ -126,10 +127,9 @@ struct Walk {
         }
       }
       const int tiles = cls == 2 ? p.tiles_o : p.tiles_p;
-      seg = static_cast<int>(pos / tiles);
-      t = static_cast<int>(pos - static_cast<int64_t>(seg) * tiles);
-      const int64_t left = end - pos;
-      const int take = tiles - t < left ? tiles - t : static_cast<int>(left);
+      seg = pos / tiles;
+      t = pos - seg * tiles;
+      const int take = min(tiles - t, end - pos);
       pos += take;
       const int per = cls == 0 ? p.pairs : (cls == 1 ? 1 : p.own_blocks);
       const int x = seg / per;
@@ -192,15 +192,34 @@ struct Steps {
 };
 struct Stateless {};
 
+// Slots of the K / V ring: as many as fit (160 of 227 KB with two query blocks of 32 KB at D = 128). A tile is read about
+// 1.6 us after its slot came free, in which the SM should have received 70 KB: two slots a K and a V of their own left
+// the ring waiting (84 us for 32 rows on a 16k prefix).
+template <int D>
+constexpr int kSlots = D == 128 ? 5 : 8;
+
 struct SpaBars {
-  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];
+  uint64_t full[8], empty[8];
   uint64_t q_full[2], q_empty[2], s_full[2], p_full[2], o_full[2];   // by stream
 };
 
 template <int D>
 constexpr int spa_smem() {
-  return 6 * kT * D * 2 + 256 + 1024;
+  return (2 + kSlots<D>) * kT * D * 2 + 256 + 1024;
 }
+
+// position in the ring
+template <int N>
+struct Ring {
+  int slot = 0;
+  uint32_t phase = 0;
+  __device__ __forceinline__ void step() {
+    if (++slot == N) {
+      slot = 0;
+      phase ^= 1u;
+    }
+  }
+};
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kSpaThreads, 1)
@@ -211,9 +230,8 @@ __global__ void __launch_bounds__(kSpaThreads, 1)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sQ = smem;                       // one block a stream
-  uint8_t* sK = sQ + 2 * kTile;             // ring
-  uint8_t* sV = sK + 2 * kTile;
-  SpaBars* bars = reinterpret_cast<SpaBars*>(sV + 2 * kTile);
+  uint8_t* sKV = sQ + 2 * kTile;            // ring
+  SpaBars* bars = reinterpret_cast<SpaBars*>(sKV + kSlots<D> * kTile);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
@@ -238,49 +256,74 @@ __global__ void __launch_bounds__(kSpaThreads, 1)
   if (warp == 0) {
     // ------------------------------------------------------------------------------------------------ K / V loads
     if (lane == 0) {
-      Steps<Stateless> st;
+      struct Tile {
+        bool pending = false;                // the V tile of the stream's last step is still to be loaded
+        int own = 0, row = 0, hk = 0, key = 0, rows = 0;
+      };
+      Steps<Tile> st;
       st.start(p, cta);
-      int nk = 0, nv = 0;
+      Ring<kSlots<D>> ring;
+      int n = 0;
+      auto load = [&](const Tile& x, const CUtensorMap* prefix, const CUtensorMap* own) -> bool {
+        uint64_t* bar = &bars->full[ring.slot];
+        if (!mbar_wait(&bars->empty[ring.slot], ring.phase ^ 1u, abort_flag, p.status, 700)) return false;
+        uint8_t* dst = sKV + ring.slot * kTile;
+        const CUtensorMap* m = x.own ? own : prefix;
+        const int box = x.own ? kOwnBox : kT;
+        const int boxes = (x.rows + box - 1) / box;
+        mbar_arrive_expect_tx(bar, boxes * box * D * 2);
+        for (int j = 0; j < boxes; ++j)
+#pragma unroll
+          for (int a = 0; a < D / 64; ++a)
+            tma_load_4d(dst + a * kAtom + j * box * 128, m, bar, a * 64, x.hk, x.key + j * box, x.row);
+        ring.step();
+        ++n;
+        return true;
+      };
+      auto load_v = [&](Tile& x) -> bool {
+        if (!x.pending) return true;
+        x.pending = false;
+        return load(x, &tm_pv, &tm_v);
+      };
+      bool ok = true;
       for (; st.live; st.advance(p, cta)) {
+        if (!(ok = load_v(st.s) && (st.live_other || load_v(st.s_other)))) break;
         if (st.follows()) continue;
         const Walk& x = st.w;
-        const int slot = nk & 1;
-        const uint32_t ph = ((nk >> 1) & 1) ^ 1u;
-        const int boxes = (min(kT, x.len - x.t * kT) + kBox - 1) / kBox;
-        const uint32_t bytes = boxes * kBox * D * 2;
-        auto load = [&](uint8_t* dst, const CUtensorMap* m, uint64_t* bar) {
-          mbar_arrive_expect_tx(bar, bytes);
-          for (int j = 0; j < boxes; ++j)
-#pragma unroll
-            for (int a = 0; a < D / 64; ++a)
-              tma_load_4d(dst + a * kAtom + j * kBox * 128, m, bar, a * 64, x.hk, x.t * kT + j * kBox, x.row);
-        };
-        if (!mbar_wait(&bars->k_empty[slot], ph, abort_flag, p.status, 700)) break;
-        load(sK + slot * kTile, x.cls == 2 ? &tm_k : &tm_pk, &bars->k_full[slot]);
-        ++nk;
-        if (!mbar_wait(&bars->v_empty[slot], ph, abort_flag, p.status, 701)) break;
-        load(sV + slot * kTile, x.cls == 2 ? &tm_v : &tm_pv, &bars->v_full[slot]);
-        ++nv;
+        st.s = Tile{true, x.cls == 2, x.row, x.hk, x.t * kT, min(kT, x.len - x.t * kT)};
+        if (!(ok = load(st.s, &tm_pk, &tm_k))) break;
       }
+      if (ok) ok = load_v(st.s_other) && load_v(st.s);
       // before the CTA ends its loads have landed, and without a timeout have been read
-      for (int i = max(nk - 2, 0); i < nk; ++i) mbar_wait(&bars->k_full[i & 1], (i >> 1) & 1, nullptr, p.status, 702);
-      for (int i = max(nv - 2, 0); i < nv; ++i) mbar_wait(&bars->v_full[i & 1], (i >> 1) & 1, nullptr, p.status, 703);
-      for (int i = max(nk - 2, 0); i < nk && !*abort_flag; ++i)
-        mbar_wait(&bars->k_empty[i & 1], (i >> 1) & 1, abort_flag, p.status, 704);
-      for (int i = max(nv - 2, 0); i < nv && !*abort_flag; ++i)
-        mbar_wait(&bars->v_empty[i & 1], (i >> 1) & 1, abort_flag, p.status, 705);
+      const int left = min(n, kSlots<D>);
+      for (int pass = 0; pass < 2; ++pass) {
+        Ring<kSlots<D>> r = ring;
+        for (int i = 0; i < left; ++i) {     // backwards: the last load is one position before `ring`
+          if (r.slot == 0) {
+            r.slot = kSlots<D>;
+            r.phase ^= 1u;
+          }
+          --r.slot;
+          if (pass == 0)
+            mbar_wait(&bars->full[r.slot], r.phase, nullptr, p.status, 702);
+          else if (!*abort_flag)
+            mbar_wait(&bars->empty[r.slot], r.phase, abort_flag, p.status, 703);
+        }
+      }
     }
   } else if (warp == 1) {
     // --------------------------------------------------------------------------------------------- matrix products
     struct Product {
       bool pending = false, first = true;    // P V of the stream's last tile is still to be issued; a piece starts
-      bool opens, last, frees, fix;          // of that product: first / last of its piece, last reader of its V tile
-      int slot, nv;
-      uint32_t vph, pph = 0, qph = 0;
+      bool opens = false, last = false;      // of that product: first / last of its piece
+      bool frees = false, follows = false;   // last / second reader of its V tile
+      int nv = 0;                            // keys of that tile
+      uint32_t pph = 0, qph = 0;
     };
     Steps<Product> st;
     st.start(p, cta);
-    int n = 0;                               // loads met so far
+    Ring<kSlots<D>> ring;
+    int k_slot = 0, v_slot = 0;              // of the last K / V tile met, for the stream that follows
     bool ok = true;
     auto wait = [&](uint64_t* bar, uint32_t ph, int site) -> bool {
       int good = 1;
@@ -290,13 +333,18 @@ __global__ void __launch_bounds__(kSpaThreads, 1)
       return good != 0;
     };
     auto issue_pv = [&](Product& v, int s) -> bool {
+      if (!v.pending) return true;
       v.pending = false;
       if (!wait(&bars->p_full[s], v.pph, 710)) return false;
       v.pph ^= 1u;
-      if (!wait(&bars->v_full[v.slot], v.vph, 711)) return false;
-      uint8_t* tile = sV + v.slot * kTile;
+      if (!v.follows) {
+        if (!wait(&bars->full[ring.slot], ring.phase, 711)) return false;
+        v_slot = ring.slot;
+        ring.step();
+      }
+      uint8_t* tile = sKV + v_slot * kTile;
       const int steps = (v.nv + 15) / 16;
-      if (v.fix && v.nv < steps * 16) {
+      if (!v.follows && v.nv < steps * 16) {
         // a weight of zero times what lies behind the last key in use has to be zero (whole rows: no swizzle)
         for (int c = lane; c < (steps * 16 - v.nv) * (D / 8); c += 32) {
           const int r = v.nv + c / (D / 8), ch = c % (D / 8);
@@ -311,27 +359,24 @@ __global__ void __launch_bounds__(kSpaThreads, 1)
         for (int k = 0; k < steps; ++k)
           umma_bf16_ts(tmem + 256 + 128 * s, tmem + 128 * s + k * 8, desc_mn(a, k), idesc_of<T>(D, true),
                        (v.opens && k == 0) ? 0u : 1u);
-        if (v.frees) umma_commit(&bars->v_empty[v.slot]);
+        if (v.frees) umma_commit(&bars->empty[v_slot]);
         if (v.last) umma_commit(&bars->o_full[s]);
       }
       __syncwarp();
       return true;
     };
-    for (; ok && st.live; st.advance(p, cta)) {
+    for (; st.live; st.advance(p, cta)) {
       const int s = st.turn;
       const Walk& x = st.w;
-      if (st.s.pending && !(ok = issue_pv(st.s, s))) break;
       // a stream that has ended must not hold its V tile while the other goes on (its product is the younger one)
-      if (!st.live_other && st.s_other.pending && !(ok = issue_pv(st.s_other, s ^ 1))) break;
+      if (!(ok = issue_pv(st.s, s) && (st.live_other || issue_pv(st.s_other, s ^ 1)))) break;
       const bool follows = st.follows();
-      const int ring = follows ? n - 1 : n;
-      const int slot = ring & 1;
-      const uint32_t ph = (ring >> 1) & 1;
       const int nv = min(kT, x.len - x.t * kT);
       const bool last = x.t + 1 >= x.t1, frees = x.cls != 0 || follows;
       if (!follows) {
-        if (!(ok = wait(&bars->k_full[slot], ph, 712))) break;
-        ++n;
+        if (!(ok = wait(&bars->full[ring.slot], ring.phase, 712))) break;
+        k_slot = ring.slot;
+        ring.step();
       }
       if (st.s.first) {
         if (!(ok = wait(&bars->q_full[s], st.s.qph, 713))) break;
@@ -339,12 +384,12 @@ __global__ void __launch_bounds__(kSpaThreads, 1)
       }
       if (lane == 0) {
         tc_fence_after();
-        const uint32_t aq = smem_u32(sQ + s * kTile), ak = smem_u32(sK + slot * kTile);
+        const uint32_t aq = smem_u32(sQ + s * kTile), ak = smem_u32(sKV + k_slot * kTile);
         const uint32_t id = idesc_of<T>((nv + 15) / 16 * 16, false);
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) umma_bf16(tmem + 128 * s, desc_k(aq, k), desc_k(ak, k), id, k > 0 ? 1u : 0u);
         umma_commit(&bars->s_full[s]);
-        if (frees) umma_commit(&bars->k_empty[slot]);
+        if (frees) umma_commit(&bars->empty[k_slot]);
         if (last) umma_commit(&bars->q_empty[s]);
       }
       __syncwarp();
@@ -352,56 +397,41 @@ __global__ void __launch_bounds__(kSpaThreads, 1)
       st.s.opens = st.s.first;
       st.s.last = last;
       st.s.frees = frees;
-      st.s.fix = !follows;
-      st.s.slot = slot;
+      st.s.follows = follows;
       st.s.nv = nv;
-      st.s.vph = ph;
       st.s.first = last;
     }
     // the products left over: the stream that did not take the last step holds the older one
-    if (ok && st.s_other.pending) ok = issue_pv(st.s_other, st.turn ^ 1);
-    if (ok && st.s.pending) ok = issue_pv(st.s, st.turn);
-  } else if (warp == 2) {
+    if (ok) ok = issue_pv(st.s_other, st.turn ^ 1) && issue_pv(st.s, st.turn);
+  } else if (warp < 4) {
     // ----------------------------------------------------------------------------------------------- query blocks
-    struct Pieces {
-      bool first = true;
-      int n = 0;
-    };
-    Steps<Pieces> st;
-    st.start(p, cta);
-    bool ok = true;
-    for (; st.live; st.advance(p, cta)) {
-      const int s = st.turn;
-      const Walk& x = st.w;
-      if (st.s.first) {
-        int good = 1;
-        if (lane == 0) good = mbar_wait(&bars->q_empty[s], (st.s.n & 1) ^ 1u, abort_flag, p.status, 720) ? 1 : 0;
-        if (!(ok = __shfl_sync(0xffffffffu, good, 0) != 0)) break;
-        __syncwarp();
-        const int chunks = x.rows(p) * (D / 8);
-        for (int c = lane; c < chunks; c += 32) {
-          const int r = c / (D / 8), ch = c % (D / 8);
-          int b, i, h;
-          x.locate(p, r, b, i, h);
-          const T* src = reinterpret_cast<const T*>(p.q.p) + b * p.q.s0 + i * p.q.s1 + h * p.q.s2 + ch * 8;
-          cp_async16(sQ + s * kTile + (ch >> 3) * kAtom + r * 128 + (((ch & 7) ^ (r & 7)) << 4), src);
-        }
-        cp_async_wait_all();
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&bars->q_full[s]);
-        ++st.s.n;
+    const int s = warp - 2;
+    Walk x;
+    uint32_t ph = 1;
+    bool any = false, ok = true;
+    while (ok && x.next_piece(p, cta, s)) {
+      if (!(ok = mbar_wait(&bars->q_empty[s], ph, abort_flag, p.status, 720))) break;
+      ph ^= 1u;
+      any = true;
+      // a lane copies whole rows: 16-byte pieces at consecutive addresses, one address computation a row
+      const int rows = x.rows(p);
+      for (int r = lane; r < rows; r += 32) {
+        int b, i, h;
+        x.locate(p, r, b, i, h);
+        const T* src = reinterpret_cast<const T*>(p.q.p) + b * p.q.s0 + i * p.q.s1 + h * p.q.s2;
+        uint8_t* dst = sQ + s * kTile + r * 128;
+#pragma unroll
+        for (int c = 0; c < D / 8; ++c) cp_async16(dst + (c >> 3) * kAtom + (((c & 7) ^ (r & 7)) << 4), src + c * 8);
       }
-      st.s.first = x.t + 1 >= x.t1;
+      cp_async_wait_all();
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars->q_full[s]);
     }
-    if (ok && lane == 0) {
-      if (st.s.n > 0) mbar_wait(&bars->q_empty[st.turn], (st.s.n - 1) & 1, abort_flag, p.status, 721);
-      if (st.s_other.n > 0)
-        mbar_wait(&bars->q_empty[st.turn ^ 1], (st.s_other.n - 1) & 1, abort_flag, p.status, 722);
-    }
+    if (ok && any) mbar_wait(&bars->q_empty[s], ph, abort_flag, p.status, 721);
   } else {
     // ---------------------------------------------------------------------------------------------------- softmax
-    const int s = warp >= 7 ? 1 : 0;
+    const int s = (warp - 4) >> 2;
     const int quad = warp & 3;
     const int r = quad * 32 + lane;
     const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
@@ -415,33 +445,40 @@ __global__ void __launch_bounds__(kSpaThreads, 1)
     while (ok && x.next_piece(p, cta, s)) {
       const int rows = x.rows(p);
       const bool active = quad * 32 < rows;              // this warp has rows
-      int b, i, h;
-      x.locate(p, min(r, rows - 1), b, i, h);
       // keys that this row sees: all in use of a prefix, of its own those up to its position
-      const int sees = x.cls == 2 ? min(x.len, x.len - p.Lq + i + 1) : x.len;
+      int sees = x.len;
+      if (x.cls == 2) {
+        int b, i, h;
+        x.locate(p, min(r, rows - 1), b, i, h);
+        sees = min(sees, x.len - p.Lq + i + 1);
+      }
       float m_ref = -INFINITY, l = 0.f;
       for (; x.t < x.t1; ++x.t) {
         if (!(ok = mbar_wait(&bars->s_full[s], s_ph, abort_flag, p.status, 730))) break;
         s_ph ^= 1u;
         if (active) {
           tc_fence_after();
-          const int nv = min(kT, x.len - x.t * kT), vis = sees - x.t * kT;
-          uint32_t v[4][32];
-#pragma unroll
-          for (int c = 0; c < 4; ++c)
-            if (c * 32 < nv) tmem_ld32(tS + c * 32, v[c]);
-          tmem_ld_wait();
+          // S is read twice, 64 columns at a time: a row of 128 in registers spills, and the loops stay small enough
+          // for the instruction cache of warps that run alone
+          const int vis = sees - x.t * kT, halves = (min(kT, x.len - x.t * kT) + 63) / 64;
           float mx = -INFINITY;
+#pragma unroll 1
+          for (int c = 0; c < halves; ++c) {
+            uint32_t v[2][32];
+            tmem_ld32(tS + c * 64, v[0]);
+            tmem_ld32(tS + c * 64 + 32, v[1]);
+            tmem_ld_wait();
+            float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            const int lim = vis - c * 64;
+            if (lim >= 64) {
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            if (c * 32 >= nv) continue;
-            if (vis < c * 32 + 32) {
+              for (int j = 0; j < 64; ++j) m4[j & 3] = fmaxf(m4[j & 3], __uint_as_float(v[j >> 5][j & 31]));
+            } else {
 #pragma unroll
-              for (int j = 0; j < 32; ++j)
-                if (c * 32 + j >= vis) v[c][j] = __float_as_uint(-INFINITY);
+              for (int j = 0; j < 64; ++j)
+                m4[j & 3] = fmaxf(m4[j & 3], j < lim ? __uint_as_float(v[j >> 5][j & 31]) : -INFINITY);
             }
-#pragma unroll
-            for (int j = 0; j < 32; ++j) mx = fmaxf(mx, __uint_as_float(v[c][j]));
+            mx = fmaxf(mx, fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])));
           }
           const float m_cand = fmaxf(m_ref, mx * p.scale_log2);
           const bool need = m_cand > m_ref + kRescaleLog2;
@@ -449,31 +486,44 @@ __global__ void __launch_bounds__(kSpaThreads, 1)
           if (__any_sync(0xffffffffu, scale_o)) {
             // the products up to the previous tile are complete: S, which this thread waited for, was issued after them
             const float f = scale_o ? fast_exp2(m_ref - m_cand) : 1.0f;
-#pragma unroll
-            for (int c = 0; c < D; c += 16) {
-              uint32_t w[16];
-              tmem_ld16(tO + c, w);
+#pragma unroll 1
+            for (int c = 0; c < D; c += 32) {
+              uint32_t w[32];
+              tmem_ld32(tO + c, w);
               tmem_ld_wait();
 #pragma unroll
-              for (int j = 0; j < 16; ++j) w[j] = __float_as_uint(__uint_as_float(w[j]) * f);
-              tmem_st16(tO + c, w);
+              for (int j = 0; j < 32; ++j) w[j] = __float_as_uint(__uint_as_float(w[j]) * f);
+              tmem_st32(tO + c, w);
             }
             if (scale_o) l *= f;
           }
           if (need) m_ref = m_cand;
           const float m = m_ref == -INFINITY ? 0.f : m_ref - kLift;
+          __syncwarp();
+#pragma unroll 1
+          for (int c = 0; c < halves; ++c) {
+            uint32_t v[2][32], w[32];
+            tmem_ld32(tS + c * 64, v[0]);
+            tmem_ld32(tS + c * 64 + 32, v[1]);
+            tmem_ld_wait();
+            const int lim = vis - c * 64;
+            if (lim < 64) {
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            if (c * 32 >= nv) continue;
-            uint32_t w[16];
+              for (int j = 0; j < 64; ++j)
+                if (j >= lim) v[j >> 5][j & 31] = __float_as_uint(-INFINITY);
+            }
+            float l4[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int j = 0; j < 16; ++j) {
-              const float a = fast_exp2(__uint_as_float(v[c][2 * j]) * p.scale_log2 - m);
-              const float e = fast_exp2(__uint_as_float(v[c][2 * j + 1]) * p.scale_log2 - m);
-              l += a + e;
+            for (int j = 0; j < 32; ++j) {
+              const float a = fast_exp2(__uint_as_float(v[j >> 4][2 * (j & 15)]) * p.scale_log2 - m);
+              const float e = fast_exp2(__uint_as_float(v[j >> 4][2 * (j & 15) + 1]) * p.scale_log2 - m);
+              l4[(2 * j) & 3] += a;
+              l4[(2 * j + 1) & 3] += e;
               w[j] = pack2<T>(a, e);
             }
-            tmem_st16(tS + c * 16, w);
+            l += (l4[0] + l4[1]) + (l4[2] + l4[3]);
+            __syncwarp();
+            tmem_st32(tS + c * 32, w);
           }
           tmem_st_wait();
           tc_fence_before();
@@ -489,7 +539,7 @@ __global__ void __launch_bounds__(kSpaThreads, 1)
                                         : static_cast<int64_t>(x.range) + x.seg;
         const int64_t at = slot * p.part_rows[x.cls] + r;
         float* dst = p.part[x.cls] + at * D;
-#pragma unroll
+#pragma unroll 1
         for (int c = 0; c < D; c += 32) {
           uint32_t v[32];
           tmem_ld32(tO + c, v);
@@ -499,8 +549,8 @@ __global__ void __launch_bounds__(kSpaThreads, 1)
             for (int j = 0; j < 8; ++j)
               *reinterpret_cast<uint4*>(dst + c + 4 * j) = make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
           }
+          __syncwarp();
         }
-        __syncwarp();
         if (r < rows) p.stat[x.cls][at] = make_float2(m_ref - kLift, l);
         tc_fence_before();
       }
@@ -515,89 +565,111 @@ __global__ void __launch_bounds__(kSpaThreads, 1)
   }
 }
 
-// Joins the pieces of each output row (a warp a row): o = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i.
+// Joins the pieces of each output row: o = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i. A block a row: its warps take
+// the pieces in turn, so that a row of forty pieces has four times ten loads in flight, and join their sums at the end.
 template <typename T, int D>
-__global__ void __launch_bounds__(128) spa_join_kernel(const __grid_constant__ PrefixParams p) {
+__global__ void __launch_bounds__(kJoinWarps * 32) spa_join_kernel(const __grid_constant__ PrefixParams p) {
   constexpr int E = D / 32;
-  const int64_t w = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
-  const int lane = threadIdx.x & 31;
-  if (w >= static_cast<int64_t>(p.B) * p.Lq * p.Hq) return;
-  const int h = static_cast<int>(w % p.Hq);
-  const int64_t tok = w / p.Hq;
+  __shared__ float sO[kJoinWarps][D];
+  __shared__ float2 sML[kJoinWarps];
+  const int64_t row = blockIdx.x;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int h = static_cast<int>(row % p.Hq);
+  const int64_t tok = row / p.Hq;
   const int i = static_cast<int>(tok % p.Lq), b = static_cast<int>(tok / p.Lq);
   const int hk = h / p.rep, n = p.B / p.G, g = b / n;
 
-  float M = -INFINITY, L = 0.f, o[E];
-#pragma unroll
-  for (int e = 0; e < E; ++e) o[e] = 0.f;
   // pieces lo .. hi of class c: slot = mul * (range + seg) + add, row r of the slot
-  auto join = [&](int c, int seg, int tiles, int used, int mul, int add, int r) {
-    if (used == 0) return;
-    const int64_t t0 = static_cast<int64_t>(seg) * tiles;
-    const int lo = static_cast<int>(range_of(t0, p.total[c], p.units[c]));
-    const int hi = static_cast<int>(range_of(t0 + used - 1, p.total[c], p.units[c]));
-    for (int base = lo; base <= hi; base += 32) {
-      const int cnt = min(32, hi + 1 - base);
-      float2 ml = make_float2(-INFINITY, 0.f);
-      if (lane < cnt)
-        ml = p.stat[c][(mul * (static_cast<int64_t>(base) + lane + seg) + add) * p.part_rows[c] + r];
-      float mx = ml.y > 0.f ? ml.x : -INFINITY;
-#pragma unroll
-      for (int x = 16; x > 0; x >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
-      if (mx == -INFINITY) continue;
-      const float Mn = fmaxf(M, mx);
-      const float f0 = M == -INFINITY ? 0.f : exp2f(M - Mn);
-      const float f = ml.y > 0.f ? exp2f(ml.x - Mn) : 0.f;
-      float lw = f * ml.y;
-#pragma unroll
-      for (int x = 16; x > 0; x >>= 1) lw += __shfl_xor_sync(0xffffffffu, lw, x);
-      L = L * f0 + lw;
-      M = Mn;
-#pragma unroll
-      for (int e = 0; e < E; ++e) o[e] *= f0;
-      for (int j = 0; j < cnt; ++j) {
-        const float fj = __shfl_sync(0xffffffffu, f, j);
-        const float* src =
-            p.part[c] + ((mul * (static_cast<int64_t>(base) + j + seg) + add) * p.part_rows[c] + r) * D + lane * E;
-        if constexpr (E == 4) {
-          const float4 t = *reinterpret_cast<const float4*>(src);
-          if (fj != 0.f) {
-            o[0] += fj * t.x;
-            o[1] += fj * t.y;
-            o[2] += fj * t.z;
-            o[3] += fj * t.w;
-          }
-        } else {
-          const float2 t = *reinterpret_cast<const float2*>(src);
-          if (fj != 0.f) {
-            o[0] += fj * t.x;
-            o[1] += fj * t.y;
-          }
-        }
-      }
+  struct List {
+    int c, lo, cnt, seg, mul, add, r;
+  } list[2];
+  auto find = [&](int c, int seg, int tiles, int used, int mul, int add, int r) -> List {
+    List x{c, 0, 0, seg, mul, add, r};
+    if (used > 0) {
+      const int64_t t0 = static_cast<int64_t>(seg) * tiles;
+      x.lo = range_of(t0, p.total[c], p.units[c]);
+      x.cnt = range_of(t0 + used - 1, p.total[c], p.units[c]) + 1 - x.lo;
     }
+    return x;
   };
   {
     const int flat = ((b - g * n) * p.Lq + i) * p.rep + h - hk * p.rep;
     const int blk = flat / kT, r = flat - blk * kT, gh = g * p.Hk + hk;
     const int used = (length_of(p.prefix_lengths, p.prefix_lengths_64, g, p.P) + kT - 1) / kT;
-    if (blk < 2 * p.pairs)
-      join(0, gh * p.pairs + (blk >> 1), p.tiles_p, used, 2, blk & 1, r);
-    else
-      join(1, gh, p.tiles_p, used, 1, 0, r);
+    list[0] = blk < 2 * p.pairs ? find(0, gh * p.pairs + (blk >> 1), p.tiles_p, used, 2, blk & 1, r)
+                                : find(1, gh, p.tiles_p, used, 1, 0, r);
   }
   {
     const int flat = i * p.rep + h - hk * p.rep;
     const int blk = flat / kT, r = flat - blk * kT;
     const int used = (length_of(p.lengths, p.lengths_64, b, p.S) + kT - 1) / kT;
-    join(2, (b * p.Hk + hk) * p.own_blocks + blk, p.tiles_o, used, 1, 0, r);
+    list[1] = find(2, (b * p.Hk + hk) * p.own_blocks + blk, p.tiles_o, used, 1, 0, r);
   }
-  const float inv = L > 0.f ? 1.0f / L : 0.f;
-  T* op = reinterpret_cast<T*>(p.o) + w * D + lane * E;
-  if constexpr (E == 4)
-    *reinterpret_cast<uint2*>(op) = make_uint2(pack2<T>(o[0] * inv, o[1] * inv), pack2<T>(o[2] * inv, o[3] * inv));
-  else
-    *reinterpret_cast<uint32_t*>(op) = pack2<T>(o[0] * inv, o[1] * inv);
+  const int cnt = list[0].cnt + list[1].cnt;
+  float M = -INFINITY, L = 0.f, o[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) o[e] = 0.f;
+  for (int base = 0; base < cnt; base += 32 * kJoinWarps) {
+    const int k = base + lane * kJoinWarps + warp;       // this lane's piece
+    const int here = min(32, (cnt - base - warp + kJoinWarps - 1) / kJoinWarps);
+    float2 ml = make_float2(-INFINITY, 0.f);
+    const float* src = nullptr;
+    if (k < cnt) {
+      const bool own = k >= list[0].cnt;
+      const List& x = own ? list[1] : list[0];
+      const int range = x.lo + (own ? k - list[0].cnt : k);
+      const int64_t at = (x.mul * (static_cast<int64_t>(range) + x.seg) + x.add) * p.part_rows[x.c] + x.r;
+      ml = p.stat[x.c][at];
+      src = p.part[x.c] + at * D;
+    }
+    float mx = ml.y > 0.f ? ml.x : -INFINITY;
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+    const float Mn = fmaxf(M, mx);
+    const float f0 = M == -INFINITY ? 0.f : exp2f(M - Mn);
+    const float f = ml.y > 0.f ? exp2f(ml.x - Mn) : 0.f;
+    float lw = f * ml.y;
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) lw += __shfl_xor_sync(0xffffffffu, lw, d);
+    L = L * f0 + lw;
+    M = Mn;
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] *= f0;
+#pragma unroll 4
+    for (int j = 0; j < here; ++j) {
+      const float fj = __shfl_sync(0xffffffffu, f, j);
+      const float* sj = reinterpret_cast<const float*>(
+                            __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(src), j)) + lane * E;
+      float t[E];
+      if constexpr (E == 4) {
+        const float4 u = *reinterpret_cast<const float4*>(sj);
+        t[0] = u.x, t[1] = u.y, t[2] = u.z, t[3] = u.w;
+      } else {
+        const float2 u = *reinterpret_cast<const float2*>(sj);
+        t[0] = u.x, t[1] = u.y;
+      }
+#pragma unroll
+      for (int e = 0; e < E; ++e) o[e] += fj != 0.f ? fj * t[e] : 0.f;
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < E; ++e) sO[warp][lane * E + e] = o[e];
+  if (lane == 0) sML[warp] = make_float2(M, L);
+  __syncthreads();
+  if (threadIdx.x < D / 2) {
+    float top = -INFINITY, total = 0.f, x0 = 0.f, x1 = 0.f;
+#pragma unroll
+    for (int w = 0; w < kJoinWarps; ++w) top = fmaxf(top, sML[w].x);
+#pragma unroll
+    for (int w = 0; w < kJoinWarps; ++w) {
+      const float f = sML[w].y > 0.f ? exp2f(sML[w].x - top) : 0.f;
+      total += f * sML[w].y;
+      x0 += f * sO[w][2 * threadIdx.x];
+      x1 += f * sO[w][2 * threadIdx.x + 1];
+    }
+    const float inv = total > 0.f ? 1.0f / total : 0.f;
+    reinterpret_cast<uint32_t*>(p.o)[row * (D / 2) + threadIdx.x] = pack2<T>(x0 * inv, x1 * inv);
+  }
 }
 
 View view_of(const at::Tensor& t, const at::Tensor& q, const char* name) {
@@ -612,14 +684,14 @@ View view_of(const at::Tensor& t, const at::Tensor& q, const char* name) {
   return View{t.data_ptr(), t.stride(0), t.stride(1), t.stride(2)};
 }
 
-// {D, heads, keys, rows} with boxes of 64 x 1 x kBox x 1; a dimension of one element has no stride to speak of
-CUtensorMap tmap_cache(const at::Tensor& t) {
+// {D, heads, keys, rows} with boxes of 64 x 1 x box_keys x 1; a dimension of one element has no stride to speak of
+CUtensorMap tmap_cache(const at::Tensor& t, int box_keys) {
   if (t.numel() == 0) return CUtensorMap{};            // no tile of it is loaded
   CUtensorMap m;
   auto bytes = [&](int d) -> cuuint64_t { return t.size(d) > 1 ? t.stride(d) * 2 : t.size(3) * 2; };
   cuuint64_t dims[4] = {(cuuint64_t)t.size(3), (cuuint64_t)t.size(2), (cuuint64_t)t.size(1), (cuuint64_t)t.size(0)};
   cuuint64_t strides[3] = {bytes(2), bytes(1), bytes(0)};
-  cuuint32_t box[4] = {64u, 1u, (cuuint32_t)kBox, 1u};
+  cuuint32_t box[4] = {64u, 1u, (cuuint32_t)box_keys, 1u};
   cuuint32_t one[4] = {1u, 1u, 1u, 1u};
   const CUresult r = encode_fn()(
       &m, t.scalar_type() == at::kHalf ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
@@ -647,8 +719,7 @@ void launch(const CUtensorMap& pk, const CUtensorMap& pv, const CUtensorMap& k, 
   FYB_CUDA(cudaFuncSetAttribute(spa_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, spa_smem<D>()));
   spa_kernel<T, D><<<p.ctas, kSpaThreads, spa_smem<D>(), cur_stream()>>>(pk, pv, k, v, p);
   check_launch("shared_prefix_attention");
-  const int64_t rows = (int64_t)p.B * p.Lq * p.Hq;
-  spa_join_kernel<T, D><<<(rows + 3) / 4, 128, 0, cur_stream()>>>(p);
+  spa_join_kernel<T, D><<<p.B * p.Lq * p.Hq, kJoinWarps * 32, 0, cur_stream()>>>(p);
   check_launch("shared_prefix_attention (join)");
 }
 
@@ -689,9 +760,13 @@ at::Tensor shared_prefix_attention(const at::Tensor& q, const at::Tensor& pk, co
   p.tiles_p = (int)((P + kT - 1) / kT);
   p.tiles_o = (int)((S + kT - 1) / kT);
   const int64_t segs[3] = {G * Hk * p.pairs, G * Hk * p.odd, B * Hk * p.own_blocks};
-  for (int c = 0; c < 3; ++c) p.total[c] = segs[c] * (c == 2 ? p.tiles_o : p.tiles_p);
+  for (int c = 0; c < 3; ++c) {
+    const int64_t tiles = segs[c] * (c == 2 ? p.tiles_o : p.tiles_p);
+    FYB_CHECK(tiles < (1ll << 31), "shared_prefix_attention: more than 2^31 tiles");
+    p.total[c] = (int)tiles;
+  }
   p.ctas = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
-  for (int c = 0; c < 3; ++c) p.units[c] = (int)std::min<int64_t>(p.total[c], c == 0 ? p.ctas : 2 * p.ctas);
+  for (int c = 0; c < 3; ++c) p.units[c] = std::min(p.total[c], c == 0 ? p.ctas : 2 * p.ctas);
   p.shift = p.units[1] % (2 * p.ctas);
   p.lengths = length_ptr(lengths, q, B, p.lengths_64);
   p.prefix_lengths = length_ptr(prefix_lengths, q, G, p.prefix_lengths_64);
@@ -718,7 +793,8 @@ at::Tensor shared_prefix_attention(const at::Tensor& q, const at::Tensor& pk, co
     p.stat[c] = reinterpret_cast<float2*>(at_);
     at_ += rows[c] * 2;
   }
-  const CUtensorMap mpk = tmap_cache(pk), mpv = tmap_cache(pv), mk = tmap_cache(k), mv = tmap_cache(v);
+  const CUtensorMap mpk = tmap_cache(pk, kT), mpv = tmap_cache(pv, kT);
+  const CUtensorMap mk = tmap_cache(k, kOwnBox), mv = tmap_cache(v, kOwnBox);
   if (q.scalar_type() == at::kBFloat16)
     D == 64 ? launch<__nv_bfloat16, 64>(mpk, mpv, mk, mv, p) : launch<__nv_bfloat16, 128>(mpk, mpv, mk, mv, p);
   else
