@@ -83,6 +83,15 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volati
   }
 }
 
+// The same with the waiting loop in one place: for kernels of many waits, whose code should stay in the instruction cache
+static __device__ __noinline__ bool mbar_wait_loop(uint64_t* bar, uint32_t parity, volatile int* abort, int* status, int site) {
+  return mbar_wait(bar, parity, abort, status, site);
+}
+__device__ __forceinline__ bool mbar_wait_short(uint64_t* bar, uint32_t parity, volatile int* abort, int* status,
+                                                int site) {
+  return mbar_try_wait(bar, parity) || mbar_wait_loop(bar, parity, abort, status, site);
+}
+
 // ------------------------------------------------------------------------------------------------------------------
 // TMA tensor loads: each CTA loads its own tiles from this GPU's memory
 

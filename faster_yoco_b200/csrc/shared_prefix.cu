@@ -90,14 +90,6 @@ __device__ __forceinline__ constexpr uint32_t idesc_of(int N, bool b_mn) {
   return sizeof(T) == 2 && !std::is_same<T, __nv_bfloat16>::value ? d & ~((7u << 7) | (7u << 10)) : d;
 }
 
-// K-major operand of 64-wide atoms; MN-major operand whose atoms are kAtom apart
-__device__ __forceinline__ uint64_t desc_k(uint32_t base, int k16) {
-  return sw128_desc(base + (k16 >> 2) * kAtom + (k16 & 3) * 32, 16, 1024);
-}
-__device__ __forceinline__ uint64_t desc_mn(uint32_t base, int k16) {
-  return sw128_desc(base + k16 * 2048, kAtom, 1024);
-}
-
 // range w of n takes tiles [w total / n, (w + 1) total / n); n <= total, so that no range is empty
 __device__ __forceinline__ int range_begin(int64_t w, int total, int n) { return static_cast<int>(w * total / n); }
 __device__ __forceinline__ int range_of(int64_t tile, int total, int n) {
@@ -266,7 +258,7 @@ __global__ void __launch_bounds__(kSpaThreads, 1)
       int n = 0;
       auto load = [&](const Tile& x, const CUtensorMap* prefix, const CUtensorMap* own) -> bool {
         uint64_t* bar = &bars->full[ring.slot];
-        if (!mbar_wait(&bars->empty[ring.slot], ring.phase ^ 1u, abort_flag, p.status, 700)) return false;
+        if (!mbar_wait_short(&bars->empty[ring.slot], ring.phase ^ 1u, abort_flag, p.status, 700)) return false;
         uint8_t* dst = sKV + ring.slot * kTile;
         const CUtensorMap* m = x.own ? own : prefix;
         const int box = x.own ? kOwnBox : kT;
@@ -305,9 +297,9 @@ __global__ void __launch_bounds__(kSpaThreads, 1)
           }
           --r.slot;
           if (pass == 0)
-            mbar_wait(&bars->full[r.slot], r.phase, nullptr, p.status, 702);
+            mbar_wait_short(&bars->full[r.slot], r.phase, nullptr, p.status, 702);
           else if (!*abort_flag)
-            mbar_wait(&bars->empty[r.slot], r.phase, abort_flag, p.status, 703);
+            mbar_wait_short(&bars->empty[r.slot], r.phase, abort_flag, p.status, 703);
         }
       }
     }
@@ -325,12 +317,11 @@ __global__ void __launch_bounds__(kSpaThreads, 1)
     Ring<kSlots<D>> ring;
     int k_slot = 0, v_slot = 0;              // of the last K / V tile met, for the stream that follows
     bool ok = true;
+    // descriptors: a tile's own bits plus its address and the K step's offset, both in units of 16 bytes
+    const uint64_t desc_km = sw128_desc(0, 16, 1024), desc_mn = sw128_desc(0, kAtom, 1024);
+    const uint32_t q16 = smem_u32(sQ) >> 4, kv16 = smem_u32(sKV) >> 4;
     auto wait = [&](uint64_t* bar, uint32_t ph, int site) -> bool {
-      int good = 1;
-      if (lane == 0) good = mbar_wait(bar, ph, abort_flag, p.status, site) ? 1 : 0;
-      good = __shfl_sync(0xffffffffu, good, 0);
-      __syncwarp();
-      return good != 0;
+      return __all_sync(0xffffffffu, mbar_wait_short(bar, ph, abort_flag, p.status, site));
     };
     auto issue_pv = [&](Product& v, int s) -> bool {
       if (!v.pending) return true;
@@ -342,10 +333,10 @@ __global__ void __launch_bounds__(kSpaThreads, 1)
         v_slot = ring.slot;
         ring.step();
       }
-      uint8_t* tile = sKV + v_slot * kTile;
       const int steps = (v.nv + 15) / 16;
       if (!v.follows && v.nv < steps * 16) {
         // a weight of zero times what lies behind the last key in use has to be zero (whole rows: no swizzle)
+        uint8_t* tile = sKV + v_slot * kTile;
         for (int c = lane; c < (steps * 16 - v.nv) * (D / 8); c += 32) {
           const int r = v.nv + c / (D / 8), ch = c % (D / 8);
           *reinterpret_cast<uint4*>(tile + (ch >> 3) * kAtom + r * 128 + (ch & 7) * 16) = make_uint4(0, 0, 0, 0);
@@ -355,10 +346,12 @@ __global__ void __launch_bounds__(kSpaThreads, 1)
       }
       if (lane == 0) {
         tc_fence_after();
-        const uint32_t a = smem_u32(tile);
-        for (int k = 0; k < steps; ++k)
-          umma_bf16_ts(tmem + 256 + 128 * s, tmem + 128 * s + k * 8, desc_mn(a, k), idesc_of<T>(D, true),
-                       (v.opens && k == 0) ? 0u : 1u);
+        const uint64_t dv = desc_mn + kv16 + v_slot * (kTile >> 4);
+        const uint32_t tp = tmem + 128 * s, to = tmem + 256 + 128 * s;
+        umma_bf16_ts(to, tp, dv, idesc_of<T>(D, true), v.opens ? 0u : 1u);
+#pragma unroll
+        for (int k = 1; k < kT / 16; ++k)
+          if (k < steps) umma_bf16_ts(to, tp + k * 8, dv + k * 128, idesc_of<T>(D, true), 1u);
         if (v.frees) umma_commit(&bars->empty[v_slot]);
         if (v.last) umma_commit(&bars->o_full[s]);
       }
@@ -384,10 +377,13 @@ __global__ void __launch_bounds__(kSpaThreads, 1)
       }
       if (lane == 0) {
         tc_fence_after();
-        const uint32_t aq = smem_u32(sQ + s * kTile), ak = smem_u32(sKV + k_slot * kTile);
+        const uint64_t dq = desc_km + q16 + s * (kTile >> 4), dk = desc_km + kv16 + k_slot * (kTile >> 4);
         const uint32_t id = idesc_of<T>((nv + 15) / 16 * 16, false);
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k) umma_bf16(tmem + 128 * s, desc_k(aq, k), desc_k(ak, k), id, k > 0 ? 1u : 0u);
+        for (int k = 0; k < D / 16; ++k) {
+          const int at = (k >> 2) * (kAtom >> 4) + (k & 3) * 2;
+          umma_bf16(tmem + 128 * s, dq + at, dk + at, id, k > 0 ? 1u : 0u);
+        }
         umma_commit(&bars->s_full[s]);
         if (frees) umma_commit(&bars->empty[k_slot]);
         if (last) umma_commit(&bars->q_empty[s]);
@@ -410,7 +406,7 @@ __global__ void __launch_bounds__(kSpaThreads, 1)
     uint32_t ph = 1;
     bool any = false, ok = true;
     while (ok && x.next_piece(p, cta, s)) {
-      if (!(ok = mbar_wait(&bars->q_empty[s], ph, abort_flag, p.status, 720))) break;
+      if (!(ok = mbar_wait_short(&bars->q_empty[s], ph, abort_flag, p.status, 720))) break;
       ph ^= 1u;
       any = true;
       // a lane copies whole rows: 16-byte pieces at consecutive addresses, one address computation a row
@@ -428,7 +424,7 @@ __global__ void __launch_bounds__(kSpaThreads, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars->q_full[s]);
     }
-    if (ok && any) mbar_wait(&bars->q_empty[s], ph, abort_flag, p.status, 721);
+    if (ok && any) mbar_wait_short(&bars->q_empty[s], ph, abort_flag, p.status, 721);
   } else {
     // ---------------------------------------------------------------------------------------------------- softmax
     const int s = (warp - 4) >> 2;
@@ -439,6 +435,14 @@ __global__ void __launch_bounds__(kSpaThreads, 1)
     // fp16 weights are lifted by 2^7 (at most 2^15 with the lazy maximum), which keeps what lies down to 2^-21 of the
     // largest in its normal range; bf16 has fp32's range
     constexpr float kLift = std::is_same<T, __half>::value ? 7.0f : 0.0f;
+    // scores of the keys behind the first n
+    auto hide = [](uint32_t (&v)[32], int n) {
+      if (__any_sync(0xffffffffu, n < 32)) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+          if (j >= n) v[j] = __float_as_uint(-INFINITY);
+      }
+    };
     Walk x;
     uint32_t s_ph = 0, o_ph = 0;
     bool ok = true;
@@ -454,31 +458,24 @@ __global__ void __launch_bounds__(kSpaThreads, 1)
       }
       float m_ref = -INFINITY, l = 0.f;
       for (; x.t < x.t1; ++x.t) {
-        if (!(ok = mbar_wait(&bars->s_full[s], s_ph, abort_flag, p.status, 730))) break;
+        if (!(ok = mbar_wait_short(&bars->s_full[s], s_ph, abort_flag, p.status, 730))) break;
         s_ph ^= 1u;
         if (active) {
           tc_fence_after();
-          // S is read twice, 64 columns at a time: a row of 128 in registers spills, and the loops stay small enough
-          // for the instruction cache of warps that run alone
-          const int vis = sees - x.t * kT, halves = (min(kT, x.len - x.t * kT) + 63) / 64;
+          // S is read twice, 32 columns at a time: a row of 128 in registers spills, and a warp that runs alone is bound
+          // by the fetching of its instructions, so the loops are kept short
+          const int vis = sees - x.t * kT, nc = (min(kT, x.len - x.t * kT) + 31) / 32;
           float mx = -INFINITY;
 #pragma unroll 1
-          for (int c = 0; c < halves; ++c) {
-            uint32_t v[2][32];
-            tmem_ld32(tS + c * 64, v[0]);
-            tmem_ld32(tS + c * 64 + 32, v[1]);
+          for (int c = 0; c < nc; ++c) {
+            uint32_t v[32];
+            tmem_ld32(tS + c * 32, v);
             tmem_ld_wait();
-            float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-            const int lim = vis - c * 64;
-            if (lim >= 64) {
+            hide(v, vis - c * 32);
+            float m4[4] = {mx, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-              for (int j = 0; j < 64; ++j) m4[j & 3] = fmaxf(m4[j & 3], __uint_as_float(v[j >> 5][j & 31]));
-            } else {
-#pragma unroll
-              for (int j = 0; j < 64; ++j)
-                m4[j & 3] = fmaxf(m4[j & 3], j < lim ? __uint_as_float(v[j >> 5][j & 31]) : -INFINITY);
-            }
-            mx = fmaxf(mx, fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])));
+            for (int j = 0; j < 32; ++j) m4[j & 3] = fmaxf(m4[j & 3], __uint_as_float(v[j]));
+            mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
           }
           const float m_cand = fmaxf(m_ref, mx * p.scale_log2);
           const bool need = m_cand > m_ref + kRescaleLog2;
@@ -500,38 +497,31 @@ __global__ void __launch_bounds__(kSpaThreads, 1)
           if (need) m_ref = m_cand;
           const float m = m_ref == -INFINITY ? 0.f : m_ref - kLift;
           __syncwarp();
+          float l4[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
-          for (int c = 0; c < halves; ++c) {
-            uint32_t v[2][32], w[32];
-            tmem_ld32(tS + c * 64, v[0]);
-            tmem_ld32(tS + c * 64 + 32, v[1]);
+          for (int c = 0; c < nc; ++c) {
+            uint32_t v[32], w[16];
+            tmem_ld32(tS + c * 32, v);
             tmem_ld_wait();
-            const int lim = vis - c * 64;
-            if (lim < 64) {
+            hide(v, vis - c * 32);
 #pragma unroll
-              for (int j = 0; j < 64; ++j)
-                if (j >= lim) v[j >> 5][j & 31] = __float_as_uint(-INFINITY);
-            }
-            float l4[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int j = 0; j < 32; ++j) {
-              const float a = fast_exp2(__uint_as_float(v[j >> 4][2 * (j & 15)]) * p.scale_log2 - m);
-              const float e = fast_exp2(__uint_as_float(v[j >> 4][2 * (j & 15) + 1]) * p.scale_log2 - m);
+            for (int j = 0; j < 16; ++j) {
+              const float a = fast_exp2(__uint_as_float(v[2 * j]) * p.scale_log2 - m);
+              const float e = fast_exp2(__uint_as_float(v[2 * j + 1]) * p.scale_log2 - m);
               l4[(2 * j) & 3] += a;
               l4[(2 * j + 1) & 3] += e;
               w[j] = pack2<T>(a, e);
             }
-            l += (l4[0] + l4[1]) + (l4[2] + l4[3]);
-            __syncwarp();
-            tmem_st32(tS + c * 32, w);
+            tmem_st16(tS + c * 16, w);      // over columns that have been read
           }
+          l += (l4[0] + l4[1]) + (l4[2] + l4[3]);
           tmem_st_wait();
           tc_fence_before();
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars->p_full[s]);
       }
-      if (!ok || !(ok = mbar_wait(&bars->o_full[s], o_ph, abort_flag, p.status, 731))) break;
+      if (!ok || !(ok = mbar_wait_short(&bars->o_full[s], o_ph, abort_flag, p.status, 731))) break;
       o_ph ^= 1u;
       if (active) {
         tc_fence_after();
