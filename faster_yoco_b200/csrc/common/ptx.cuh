@@ -257,6 +257,14 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
       : "memory");
 }
 
+// true in one lane of a converged warp, always the same one. Unlike a test of the lane number it leaves the compiler
+// free to hold the operands of the issued instruction in uniform registers.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
+}
+
 // exp2 on the SFU (PTX ex2.approx.ftz.f32: relative error ~2^-22, flushes denormals; exp2(-inf) = 0)
 __device__ __forceinline__ float fast_exp2(float x) {
   float y;

@@ -53,6 +53,7 @@ struct PrefixParams {
   int pairs, odd, own_blocks;           // 128-row blocks: pairs and 0 / 1 more for the prefix, blocks of own keys
   int tiles_p, tiles_o;                 // stored tiles
   int total[3];                         // tiles of each class
+  double inv_total[3];
   int units[3];                         // ranges that each class is cut into, none of them empty
   int shift;                            // first stream that takes a range of class 2
   int ctas;
@@ -73,6 +74,11 @@ __device__ __forceinline__ int length_of(const void* p, int wide, int i, int mos
   return static_cast<int>(n < 0 ? 0 : (n > most ? most : n));
 }
 
+// a value that is the same in all lanes, as the compiler sees it
+__device__ __forceinline__ uint32_t uniform(uint32_t x) { return __shfl_sync(0xffffffffu, x, 0); }
+__device__ __forceinline__ int uniform(int x) { return __shfl_sync(0xffffffffu, x, 0); }
+__device__ __forceinline__ int uniform(bool x) { return __shfl_sync(0xffffffffu, static_cast<int>(x), 0); }
+
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi);
 template <>
@@ -92,8 +98,14 @@ __device__ __forceinline__ constexpr uint32_t idesc_of(int N, bool b_mn) {
 
 // range w of n takes tiles [w total / n, (w + 1) total / n); n <= total, so that no range is empty
 __device__ __forceinline__ int range_begin(int64_t w, int total, int n) { return static_cast<int>(w * total / n); }
-__device__ __forceinline__ int range_of(int64_t tile, int total, int n) {
-  return static_cast<int>(((tile + 1) * n - 1) / total);
+// the range that holds a tile: floor(((tile + 1) n - 1) / total), from a quotient in 64-bit floating point that is off by
+// one at most (`inv` = 1 / total) instead of a division of 64-bit integers
+__device__ __forceinline__ int range_of(int64_t tile, int total, double inv, int n) {
+  const int64_t x = (tile + 1) * n - 1;
+  int q = static_cast<int>(static_cast<double>(x) * inv);
+  if (static_cast<int64_t>(q) * total > x) --q;
+  if (static_cast<int64_t>(q + 1) * total <= x) ++q;
+  return q;
 }
 
 // The pieces of one stream in order; every role walks its own copy.
@@ -245,62 +257,70 @@ __global__ void __launch_bounds__(kSpaThreads, 1)
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;         // S of stream s (P over its first columns) @ 128 s, O @ 256 + 128 s
 
+  // a wait of a whole warp
+  auto wait = [&](uint64_t* bar, uint32_t ph, int site) -> bool {
+    return __all_sync(0xffffffffu, mbar_wait_short(bar, ph, abort_flag, p.status, site));
+  };
   if (warp == 0) {
     // ------------------------------------------------------------------------------------------------ K / V loads
-    if (lane == 0) {
-      struct Tile {
-        bool pending = false;                // the V tile of the stream's last step is still to be loaded
-        int own = 0, row = 0, hk = 0, key = 0, rows = 0;
-      };
-      Steps<Tile> st;
-      st.start(p, cta);
-      Ring<kSlots<D>> ring;
-      int n = 0;
-      auto load = [&](const Tile& x, const CUtensorMap* prefix, const CUtensorMap* own) -> bool {
-        uint64_t* bar = &bars->full[ring.slot];
-        if (!mbar_wait_short(&bars->empty[ring.slot], ring.phase ^ 1u, abort_flag, p.status, 700)) return false;
-        uint8_t* dst = sKV + ring.slot * kTile;
-        const CUtensorMap* m = x.own ? own : prefix;
-        const int box = x.own ? kOwnBox : kT;
-        const int boxes = (x.rows + box - 1) / box;
+    // the whole warp walks, one lane issues: the operands of TMA and of products live in uniform registers
+    struct Tile {
+      bool pending = false;                  // the V tile of the stream's last step is still to be loaded
+      int own = 0, row = 0, hk = 0, key = 0, rows = 0;
+    };
+    Steps<Tile> st;
+    st.start(p, cta);
+    Ring<kSlots<D>> ring;
+    int n = 0;
+    auto load = [&](const Tile& x, const CUtensorMap* prefix, const CUtensorMap* own) -> bool {
+      const int slot = uniform(ring.slot), key = uniform(x.key), hk = uniform(x.hk), row = uniform(x.row);
+      const bool is_own = uniform(x.own) != 0;
+      uint64_t* bar = &bars->full[slot];
+      if (!wait(&bars->empty[slot], ring.phase ^ 1u, 700)) return false;
+      const CUtensorMap* m = is_own ? own : prefix;
+      const int box = is_own ? kOwnBox : kT;
+      const int boxes = uniform((x.rows + box - 1) / box);
+      if (elect_one()) {
+        uint8_t* dst = sKV + slot * kTile;
         mbar_arrive_expect_tx(bar, boxes * box * D * 2);
         for (int j = 0; j < boxes; ++j)
 #pragma unroll
           for (int a = 0; a < D / 64; ++a)
-            tma_load_4d(dst + a * kAtom + j * box * 128, m, bar, a * 64, x.hk, x.key + j * box, x.row);
-        ring.step();
-        ++n;
-        return true;
-      };
-      auto load_v = [&](Tile& x) -> bool {
-        if (!x.pending) return true;
-        x.pending = false;
-        return load(x, &tm_pv, &tm_v);
-      };
-      bool ok = true;
-      for (; st.live; st.advance(p, cta)) {
-        if (!(ok = load_v(st.s) && (st.live_other || load_v(st.s_other)))) break;
-        if (st.follows()) continue;
-        const Walk& x = st.w;
-        st.s = Tile{true, x.cls == 2, x.row, x.hk, x.t * kT, min(kT, x.len - x.t * kT)};
-        if (!(ok = load(st.s, &tm_pk, &tm_k))) break;
+            tma_load_4d(dst + a * kAtom + j * box * 128, m, bar, a * 64, hk, key + j * box, row);
       }
-      if (ok) ok = load_v(st.s_other) && load_v(st.s);
-      // before the CTA ends its loads have landed, and without a timeout have been read
-      const int left = min(n, kSlots<D>);
-      for (int pass = 0; pass < 2; ++pass) {
-        Ring<kSlots<D>> r = ring;
-        for (int i = 0; i < left; ++i) {     // backwards: the last load is one position before `ring`
-          if (r.slot == 0) {
-            r.slot = kSlots<D>;
-            r.phase ^= 1u;
-          }
-          --r.slot;
-          if (pass == 0)
-            mbar_wait_short(&bars->full[r.slot], r.phase, nullptr, p.status, 702);
-          else if (!*abort_flag)
-            mbar_wait_short(&bars->empty[r.slot], r.phase, abort_flag, p.status, 703);
+      __syncwarp();
+      ring.step();
+      ++n;
+      return true;
+    };
+    auto load_v = [&](Tile& x) -> bool {
+      if (!x.pending) return true;
+      x.pending = false;
+      return load(x, &tm_pv, &tm_v);
+    };
+    bool ok = true;
+    for (; st.live; st.advance(p, cta)) {
+      if (!(ok = load_v(st.s) && (st.live_other || load_v(st.s_other)))) break;
+      if (st.follows()) continue;
+      const Walk& x = st.w;
+      st.s = Tile{true, x.cls == 2, x.row, x.hk, x.t * kT, min(kT, x.len - x.t * kT)};
+      if (!(ok = load(st.s, &tm_pk, &tm_k))) break;
+    }
+    if (ok) ok = load_v(st.s_other) && load_v(st.s);
+    // before the CTA ends its loads have landed, and without a timeout have been read
+    const int left = min(n, kSlots<D>);
+    for (int pass = 0; pass < 2; ++pass) {
+      Ring<kSlots<D>> r = ring;
+      for (int i = 0; i < left; ++i) {       // backwards: the last load is one position before `ring`
+        if (r.slot == 0) {
+          r.slot = kSlots<D>;
+          r.phase ^= 1u;
         }
+        --r.slot;
+        if (pass == 0)
+          mbar_wait_short(&bars->full[r.slot], r.phase, nullptr, p.status, 702);
+        else if (!*abort_flag)
+          mbar_wait_short(&bars->empty[r.slot], r.phase, abort_flag, p.status, 703);
       }
     }
   } else if (warp == 1) {
@@ -319,10 +339,7 @@ __global__ void __launch_bounds__(kSpaThreads, 1)
     bool ok = true;
     // descriptors: a tile's own bits plus its address and the K step's offset, both in units of 16 bytes
     const uint64_t desc_km = sw128_desc(0, 16, 1024), desc_mn = sw128_desc(0, kAtom, 1024);
-    const uint32_t q16 = smem_u32(sQ) >> 4, kv16 = smem_u32(sKV) >> 4;
-    auto wait = [&](uint64_t* bar, uint32_t ph, int site) -> bool {
-      return __all_sync(0xffffffffu, mbar_wait_short(bar, ph, abort_flag, p.status, site));
-    };
+    const uint32_t q16 = uniform(smem_u32(sQ) >> 4), kv16 = uniform(smem_u32(sKV) >> 4), tm = uniform(tmem);
     auto issue_pv = [&](Product& v, int s) -> bool {
       if (!v.pending) return true;
       v.pending = false;
@@ -344,16 +361,18 @@ __global__ void __launch_bounds__(kSpaThreads, 1)
         fence_proxy_async_smem();
         __syncwarp();
       }
-      if (lane == 0) {
-        tc_fence_after();
-        const uint64_t dv = desc_mn + kv16 + v_slot * (kTile >> 4);
-        const uint32_t tp = tmem + 128 * s, to = tmem + 256 + 128 * s;
-        umma_bf16_ts(to, tp, dv, idesc_of<T>(D, true), v.opens ? 0u : 1u);
+      const int vs = uniform(v_slot), su = uniform(s), n16 = uniform(steps);
+      const bool opens = uniform(v.opens) != 0, frees = uniform(v.frees) != 0, last = uniform(v.last) != 0;
+      tc_fence_after();
+      if (elect_one()) {
+        const uint64_t dv = desc_mn + kv16 + vs * (kTile >> 4);
+        const uint32_t tp = tm + 128 * su, to = tm + 256 + 128 * su;
+        umma_bf16_ts(to, tp, dv, idesc_of<T>(D, true), opens ? 0u : 1u);
 #pragma unroll
         for (int k = 1; k < kT / 16; ++k)
-          if (k < steps) umma_bf16_ts(to, tp + k * 8, dv + k * 128, idesc_of<T>(D, true), 1u);
-        if (v.frees) umma_commit(&bars->empty[v_slot]);
-        if (v.last) umma_commit(&bars->o_full[s]);
+          if (k < n16) umma_bf16_ts(to, tp + k * 8, dv + k * 128, idesc_of<T>(D, true), 1u);
+        if (frees) umma_commit(&bars->empty[vs]);
+        if (last) umma_commit(&bars->o_full[su]);
       }
       __syncwarp();
       return true;
@@ -375,18 +394,20 @@ __global__ void __launch_bounds__(kSpaThreads, 1)
         if (!(ok = wait(&bars->q_full[s], st.s.qph, 713))) break;
         st.s.qph ^= 1u;
       }
-      if (lane == 0) {
-        tc_fence_after();
-        const uint64_t dq = desc_km + q16 + s * (kTile >> 4), dk = desc_km + kv16 + k_slot * (kTile >> 4);
-        const uint32_t id = idesc_of<T>((nv + 15) / 16 * 16, false);
+      const int ks = uniform(k_slot), su = uniform(s);
+      const uint32_t id = uniform(idesc_of<T>((nv + 15) / 16 * 16, false));
+      const bool frees_u = uniform(frees) != 0, last_u = uniform(last) != 0;
+      tc_fence_after();
+      if (elect_one()) {
+        const uint64_t dq = desc_km + q16 + su * (kTile >> 4), dk = desc_km + kv16 + ks * (kTile >> 4);
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) {
           const int at = (k >> 2) * (kAtom >> 4) + (k & 3) * 2;
-          umma_bf16(tmem + 128 * s, dq + at, dk + at, id, k > 0 ? 1u : 0u);
+          umma_bf16(tm + 128 * su, dq + at, dk + at, id, k > 0 ? 1u : 0u);
         }
-        umma_commit(&bars->s_full[s]);
-        if (frees) umma_commit(&bars->empty[k_slot]);
-        if (last) umma_commit(&bars->q_empty[s]);
+        umma_commit(&bars->s_full[su]);
+        if (frees_u) umma_commit(&bars->empty[ks]);
+        if (last_u) umma_commit(&bars->q_empty[su]);
       }
       __syncwarp();
       st.s.pending = true;
@@ -577,8 +598,8 @@ __global__ void __launch_bounds__(kJoinWarps * 32) spa_join_kernel(const __grid_
     List x{c, 0, 0, seg, mul, add, r};
     if (used > 0) {
       const int64_t t0 = static_cast<int64_t>(seg) * tiles;
-      x.lo = range_of(t0, p.total[c], p.units[c]);
-      x.cnt = range_of(t0 + used - 1, p.total[c], p.units[c]) + 1 - x.lo;
+      x.lo = range_of(t0, p.total[c], p.inv_total[c], p.units[c]);
+      x.cnt = range_of(t0 + used - 1, p.total[c], p.inv_total[c], p.units[c]) + 1 - x.lo;
     }
     return x;
   };
@@ -754,6 +775,7 @@ at::Tensor shared_prefix_attention(const at::Tensor& q, const at::Tensor& pk, co
     const int64_t tiles = segs[c] * (c == 2 ? p.tiles_o : p.tiles_p);
     FYB_CHECK(tiles < (1ll << 31), "shared_prefix_attention: more than 2^31 tiles");
     p.total[c] = (int)tiles;
+    p.inv_total[c] = tiles > 0 ? 1.0 / (double)tiles : 0.0;
   }
   p.ctas = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
   for (int c = 0; c < 3; ++c) p.units[c] = std::min(p.total[c], c == 0 ? p.ctas : 2 * p.ctas);
