@@ -37,7 +37,7 @@ constexpr int kT = 128;                 // tile: keys, and query rows
 constexpr int kOwnBox = 32;             // key rows of one TMA box of own keys: what their last tile is rounded up to
 constexpr int kAtom = kT * 128;         // 128 rows of a 128-byte swizzle atom
 constexpr int kSpaThreads = 384;
-constexpr int kJoinWarps = 4;
+constexpr int kJoinCols = 2;            // warps of a joining block that share out the columns
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRescaleLog2 = 8.0f;
 
@@ -46,15 +46,17 @@ struct View {                           // [rows, keys, heads, D], last dim cont
   int64_t s0, s1, s2;
 };
 
+struct Cuts {
+  int units, len, rem;
+};
+
 struct PrefixParams {
   View q;
   int B, Lq, Hq, Hk, G, P, S;
   int rep, rows_p, rows_o;              // heads of a GQA group; query rows of (group, head), of (row, head)
   int pairs, odd, own_blocks;           // 128-row blocks: pairs and 0 / 1 more for the prefix, blocks of own keys
   int tiles_p, tiles_o;                 // stored tiles
-  int total[3];                         // tiles of each class
-  double inv_total[3];
-  int units[3];                         // ranges that each class is cut into, none of them empty
+  Cuts cuts[3];                         // of each class's tiles
   int shift;                            // first stream that takes a range of class 2
   int ctas;
   const void* lengths;                  // per row (int32 or int64), or null: S
@@ -62,7 +64,7 @@ struct PrefixParams {
   int lengths_64, prefix_lengths_64;
   float scale_log2;
   void* o;                              // [B, Lq, Hq, D] contiguous
-  float* part[3];                       // pieces: [slot][rows of the class][D]
+  float* part[3];                       // pieces: [slot][D / 4][rows of the class][4]
   float2* stat[3];                      // (m in log2 units, l) of each row
   int part_rows[3];
   int* status;
@@ -96,16 +98,11 @@ __device__ __forceinline__ constexpr uint32_t idesc_of(int N, bool b_mn) {
   return sizeof(T) == 2 && !std::is_same<T, __nv_bfloat16>::value ? d & ~((7u << 7) | (7u << 10)) : d;
 }
 
-// range w of n takes tiles [w total / n, (w + 1) total / n); n <= total, so that no range is empty
-__device__ __forceinline__ int range_begin(int64_t w, int total, int n) { return static_cast<int>(w * total / n); }
-// the range that holds a tile: floor(((tile + 1) n - 1) / total), from a quotient in 64-bit floating point that is off by
-// one at most (`inv` = 1 / total) instead of a division of 64-bit integers
-__device__ __forceinline__ int range_of(int64_t tile, int total, double inv, int n) {
-  const int64_t x = (tile + 1) * n - 1;
-  int q = static_cast<int>(static_cast<double>(x) * inv);
-  if (static_cast<int64_t>(q) * total > x) --q;
-  if (static_cast<int64_t>(q + 1) * total <= x) ++q;
-  return q;
+// A class's tiles in `units` ranges of len tiles, the first `rem` of them one longer; units <= tiles, so none is empty.
+__host__ __device__ __forceinline__ int range_begin(const Cuts& c, int w) { return w * c.len + min(w, c.rem); }
+__device__ __forceinline__ int range_of(const Cuts& c, int tile) {
+  const int big = c.rem * (c.len + 1);
+  return tile < big ? tile / (c.len + 1) : c.rem + (tile - big) / c.len;
 }
 
 // The pieces of one stream in order; every role walks its own copy.
@@ -125,9 +122,9 @@ struct Walk {
         // over the machine; class 2 starts behind the streams that class 1 gave work to
         range = cls == 0 ? cta : stream * p.ctas + cta;
         if (cls == 2) range = range >= p.shift ? range - p.shift : range - p.shift + 2 * p.ctas;
-        if (range < p.units[cls]) {
-          pos = range_begin(range, p.total[cls], p.units[cls]);
-          end = range_begin(range + 1, p.total[cls], p.units[cls]);
+        if (range < p.cuts[cls].units) {
+          pos = range_begin(p.cuts[cls], range);
+          end = range_begin(p.cuts[cls], range + 1);
         }
       }
       const int tiles = cls == 2 ? p.tiles_o : p.tiles_p;
@@ -336,6 +333,7 @@ __global__ void __launch_bounds__(kSpaThreads, 1)
     st.start(p, cta);
     Ring<kSlots<D>> ring;
     int k_slot = 0, v_slot = 0;              // of the last K / V tile met, for the stream that follows
+    int freed = -1;                          // slot of a V tile whose products have been issued
     bool ok = true;
     // descriptors: a tile's own bits plus its address and the K step's offset, both in units of 16 bytes
     const uint64_t desc_km = sw128_desc(0, 16, 1024), desc_mn = sw128_desc(0, kAtom, 1024);
@@ -361,27 +359,39 @@ __global__ void __launch_bounds__(kSpaThreads, 1)
         fence_proxy_async_smem();
         __syncwarp();
       }
-      const int vs = uniform(v_slot), su = uniform(s), n16 = uniform(steps);
-      const bool opens = uniform(v.opens) != 0, frees = uniform(v.frees) != 0, last = uniform(v.last) != 0;
+      const int u = uniform(v_slot | s << 4 | (v.opens ? 32 : 0) | (v.last ? 64 : 0) | steps << 8);
+      const int vs = u & 15, su = u >> 4 & 1, n16 = u >> 8;
       tc_fence_after();
       if (elect_one()) {
         const uint64_t dv = desc_mn + kv16 + vs * (kTile >> 4);
         const uint32_t tp = tm + 128 * su, to = tm + 256 + 128 * su;
-        umma_bf16_ts(to, tp, dv, idesc_of<T>(D, true), opens ? 0u : 1u);
+        umma_bf16_ts(to, tp, dv, idesc_of<T>(D, true), (u & 32) ? 0u : 1u);
 #pragma unroll
         for (int k = 1; k < kT / 16; ++k)
           if (k < n16) umma_bf16_ts(to, tp + k * 8, dv + k * 128, idesc_of<T>(D, true), 1u);
-        if (frees) umma_commit(&bars->empty[vs]);
-        if (last) umma_commit(&bars->o_full[su]);
+        if (u & 64) umma_commit(&bars->o_full[su]);
       }
       __syncwarp();
+      if (v.frees) freed = vs;
       return true;
+    };
+    // the slot of the last V tile is handed back after the next scores have been issued, so as not to hold them up
+    auto free_v = [&]() {
+      if (freed < 0) return;
+      const int vs = uniform(freed);
+      if (elect_one()) umma_commit(&bars->empty[vs]);
+      __syncwarp();
+      freed = -1;
     };
     for (; st.live; st.advance(p, cta)) {
       const int s = st.turn;
       const Walk& x = st.w;
       // a stream that has ended must not hold its V tile while the other goes on (its product is the younger one)
-      if (!(ok = issue_pv(st.s, s) && (st.live_other || issue_pv(st.s_other, s ^ 1)))) break;
+      if (!(ok = issue_pv(st.s, s))) break;
+      if (!st.live_other && st.s_other.pending) {
+        free_v();
+        if (!(ok = issue_pv(st.s_other, s ^ 1))) break;
+      }
       const bool follows = st.follows();
       const int nv = min(kT, x.len - x.t * kT);
       const bool last = x.t + 1 >= x.t1, frees = x.cls != 0 || follows;
@@ -394,9 +404,9 @@ __global__ void __launch_bounds__(kSpaThreads, 1)
         if (!(ok = wait(&bars->q_full[s], st.s.qph, 713))) break;
         st.s.qph ^= 1u;
       }
-      const int ks = uniform(k_slot), su = uniform(s);
-      const uint32_t id = uniform(idesc_of<T>((nv + 15) / 16 * 16, false));
-      const bool frees_u = uniform(frees) != 0, last_u = uniform(last) != 0;
+      const int u = uniform(k_slot | s << 4 | (frees ? 32 : 0) | (last ? 64 : 0) | (nv + 15) / 16 << 8);
+      const int ks = u & 15, su = u >> 4 & 1;
+      const uint32_t id = idesc_of<T>(0, false) | static_cast<uint32_t>(u >> 8) << 18;     // N = 16 x count
       tc_fence_after();
       if (elect_one()) {
         const uint64_t dq = desc_km + q16 + su * (kTile >> 4), dk = desc_km + kv16 + ks * (kTile >> 4);
@@ -406,10 +416,11 @@ __global__ void __launch_bounds__(kSpaThreads, 1)
           umma_bf16(tm + 128 * su, dq + at, dk + at, id, k > 0 ? 1u : 0u);
         }
         umma_commit(&bars->s_full[su]);
-        if (frees_u) umma_commit(&bars->empty[ks]);
-        if (last_u) umma_commit(&bars->q_empty[su]);
+        if (u & 32) umma_commit(&bars->empty[ks]);
+        if (u & 64) umma_commit(&bars->q_empty[su]);
       }
       __syncwarp();
+      free_v();
       st.s.pending = true;
       st.s.opens = st.s.first;
       st.s.last = last;
@@ -419,7 +430,10 @@ __global__ void __launch_bounds__(kSpaThreads, 1)
       st.s.first = last;
     }
     // the products left over: the stream that did not take the last step holds the older one
-    if (ok) ok = issue_pv(st.s_other, st.turn ^ 1) && issue_pv(st.s, st.turn);
+    if (ok) ok = issue_pv(st.s_other, st.turn ^ 1);
+    free_v();
+    if (ok) ok = issue_pv(st.s, st.turn);
+    free_v();
   } else if (warp < 4) {
     // ----------------------------------------------------------------------------------------------- query blocks
     const int s = warp - 2;
@@ -518,7 +532,8 @@ __global__ void __launch_bounds__(kSpaThreads, 1)
           if (need) m_ref = m_cand;
           const float m = m_ref == -INFINITY ? 0.f : m_ref - kLift;
           __syncwarp();
-          float l4[4] = {0.f, 0.f, 0.f, 0.f};
+          const float2 sc = make_float2(p.scale_log2, p.scale_log2), nm = make_float2(-m, -m);
+          float2 l2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll 1
           for (int c = 0; c < nc; ++c) {
             uint32_t v[32], w[16];
@@ -527,15 +542,14 @@ __global__ void __launch_bounds__(kSpaThreads, 1)
             hide(v, vis - c * 32);
 #pragma unroll
             for (int j = 0; j < 16; ++j) {
-              const float a = fast_exp2(__uint_as_float(v[2 * j]) * p.scale_log2 - m);
-              const float e = fast_exp2(__uint_as_float(v[2 * j + 1]) * p.scale_log2 - m);
-              l4[(2 * j) & 3] += a;
-              l4[(2 * j + 1) & 3] += e;
-              w[j] = pack2<T>(a, e);
+              const float2 t = fma2(make_float2(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1])), sc, nm);
+              const float2 e = make_float2(fast_exp2(t.x), fast_exp2(t.y));
+              l2[j & 1] = add2(l2[j & 1], e);
+              w[j] = pack2<T>(e.x, e.y);
             }
             tmem_st16(tS + c * 16, w);      // over columns that have been read
           }
-          l += (l4[0] + l4[1]) + (l4[2] + l4[3]);
+          l += (l2[0].x + l2[0].y) + (l2[1].x + l2[1].y);
           tmem_st_wait();
           tc_fence_before();
         }
@@ -549,7 +563,8 @@ __global__ void __launch_bounds__(kSpaThreads, 1)
         const int64_t slot = x.cls == 0 ? 2 * (static_cast<int64_t>(x.range) + x.seg) + s
                                         : static_cast<int64_t>(x.range) + x.seg;
         const int64_t at = slot * p.part_rows[x.cls] + r;
-        float* dst = p.part[x.cls] + at * D;
+        // four values of all rows side by side: the lanes of a warp, a row each, store whole lines
+        float4* dst = reinterpret_cast<float4*>(p.part[x.cls]) + slot * p.part_rows[x.cls] * (D / 4) + r;
 #pragma unroll 1
         for (int c = 0; c < D; c += 32) {
           uint32_t v[32];
@@ -558,7 +573,8 @@ __global__ void __launch_bounds__(kSpaThreads, 1)
           if (r < rows) {
 #pragma unroll
             for (int j = 0; j < 8; ++j)
-              *reinterpret_cast<uint4*>(dst + c + 4 * j) = make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+              *reinterpret_cast<uint4*>(dst + (c / 4 + j) * p.part_rows[x.cls]) =
+                  make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
           }
           __syncwarp();
         }
@@ -576,110 +592,104 @@ __global__ void __launch_bounds__(kSpaThreads, 1)
   }
 }
 
-// Joins the pieces of each output row: o = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i. A block a row: its warps take
-// the pieces in turn, so that a row of forty pieces has four times ten loads in flight, and join their sums at the end.
-template <typename T, int D>
-__global__ void __launch_bounds__(kJoinWarps * 32) spa_join_kernel(const __grid_constant__ PrefixParams p) {
-  constexpr int E = D / 32;
-  __shared__ float sO[kJoinWarps][D];
-  __shared__ float2 sML[kJoinWarps];
-  const int64_t row = blockIdx.x;
+// Joins the pieces of each output row: o = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i. A block has eight consecutive
+// rows of a (group, key / value head): its warps share them out by columns (kJoinCols) and by pieces (Parts), a lane
+// has one row and D / 32 columns in fours, so that a load of a warp covers whole 128-byte lines and a thread has its loads
+// in flight together; the parts join in shared memory.
+template <typename T, int D, int Parts>
+__global__ void __launch_bounds__(kJoinCols * Parts * 32) spa_join_kernel(const __grid_constant__ PrefixParams p) {
+  constexpr int F = D / 4 / (4 * kJoinCols);             // float4s of a lane: columns 4 (lane / 8 + 4 (wc + kJoinCols f))
+  __shared__ float4 sO[Parts - 1][D / 4][8];
+  __shared__ float2 sML[Parts][8];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int h = static_cast<int>(row % p.Hq);
-  const int64_t tok = row / p.Hq;
-  const int i = static_cast<int>(tok % p.Lq), b = static_cast<int>(tok / p.Lq);
-  const int hk = h / p.rep, n = p.B / p.G, g = b / n;
+  const int wc = warp % kJoinCols, wp = warp / kJoinCols;
+  const int per = (p.rows_p + 7) / 8;
+  const int gh = blockIdx.x / per, flat = (blockIdx.x - gh * per) * 8 + (lane & 7);
+  const bool live = flat < p.rows_p;
+  const int hk = gh % p.Hk, g = gh / p.Hk;
+  const int tok = flat / p.rep, hr = flat - tok * p.rep;
+  const int bi = tok / p.Lq, i = tok - bi * p.Lq, b = g * (p.B / p.G) + bi;
 
-  // pieces lo .. hi of class c: slot = mul * (range + seg) + add, row r of the slot
-  struct List {
-    int c, lo, cnt, seg, mul, add, r;
-  } list[2];
-  auto find = [&](int c, int seg, int tiles, int used, int mul, int add, int r) -> List {
-    List x{c, 0, 0, seg, mul, add, r};
-    if (used > 0) {
-      const int64_t t0 = static_cast<int64_t>(seg) * tiles;
-      x.lo = range_of(t0, p.total[c], p.inv_total[c], p.units[c]);
-      x.cnt = range_of(t0 + used - 1, p.total[c], p.inv_total[c], p.units[c]) + 1 - x.lo;
-    }
-    return x;
-  };
-  {
-    const int flat = ((b - g * n) * p.Lq + i) * p.rep + h - hk * p.rep;
-    const int blk = flat / kT, r = flat - blk * kT, gh = g * p.Hk + hk;
-    const int used = (length_of(p.prefix_lengths, p.prefix_lengths_64, g, p.P) + kT - 1) / kT;
-    list[0] = blk < 2 * p.pairs ? find(0, gh * p.pairs + (blk >> 1), p.tiles_p, used, 2, blk & 1, r)
-                                : find(1, gh, p.tiles_p, used, 1, 0, r);
-  }
-  {
-    const int flat = i * p.rep + h - hk * p.rep;
-    const int blk = flat / kT, r = flat - blk * kT;
-    const int used = (length_of(p.lengths, p.lengths_64, b, p.S) + kT - 1) / kT;
-    list[1] = find(2, (b * p.Hk + hk) * p.own_blocks + blk, p.tiles_o, used, 1, 0, r);
-  }
-  const int cnt = list[0].cnt + list[1].cnt;
-  float M = -INFINITY, L = 0.f, o[E];
+  float M = -INFINITY, L = 0.f;
+  float4 o[F];
 #pragma unroll
-  for (int e = 0; e < E; ++e) o[e] = 0.f;
-  for (int base = 0; base < cnt; base += 32 * kJoinWarps) {
-    const int k = base + lane * kJoinWarps + warp;       // this lane's piece
-    const int here = min(32, (cnt - base - warp + kJoinWarps - 1) / kJoinWarps);
-    float2 ml = make_float2(-INFINITY, 0.f);
-    const float* src = nullptr;
-    if (k < cnt) {
-      const bool own = k >= list[0].cnt;
-      const List& x = own ? list[1] : list[0];
-      const int range = x.lo + (own ? k - list[0].cnt : k);
-      const int64_t at = (x.mul * (static_cast<int64_t>(range) + x.seg) + x.add) * p.part_rows[x.c] + x.r;
-      ml = p.stat[x.c][at];
-      src = p.part[x.c] + at * D;
-    }
-    float mx = ml.y > 0.f ? ml.x : -INFINITY;
+  for (int f = 0; f < F; ++f) o[f] = make_float4(0.f, 0.f, 0.f, 0.f);
+  auto piece = [&](const float4* src, const float2* stat, int rows) {
+    const float2 ml = *stat;
+    float4 t[F];
 #pragma unroll
-    for (int d = 16; d > 0; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
-    const float Mn = fmaxf(M, mx);
-    const float f0 = M == -INFINITY ? 0.f : exp2f(M - Mn);
-    const float f = ml.y > 0.f ? exp2f(ml.x - Mn) : 0.f;
-    float lw = f * ml.y;
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) lw += __shfl_xor_sync(0xffffffffu, lw, d);
-    L = L * f0 + lw;
+    for (int f = 0; f < F; ++f) t[f] = src[((lane >> 3) + 4 * (wc + kJoinCols * f)) * rows];
+    const bool any = ml.y > 0.f;
+    const float Mn = any ? fmaxf(M, ml.x) : M;
+    const float f0 = M == -INFINITY ? 0.f : fast_exp2(M - Mn), w = any ? fast_exp2(ml.x - Mn) : 0.f;
     M = Mn;
+    L = L * f0 + w * ml.y;
 #pragma unroll
-    for (int e = 0; e < E; ++e) o[e] *= f0;
+    for (int f = 0; f < F; ++f) {
+      if (!any) t[f] = make_float4(0.f, 0.f, 0.f, 0.f);
+      o[f] = make_float4(o[f].x * f0 + w * t[f].x, o[f].y * f0 + w * t[f].y, o[f].z * f0 + w * t[f].z,
+                         o[f].w * f0 + w * t[f].w);
+    }
+  };
+  // pieces of the prefix: the same for the eight rows, which lie in one 128-row block
+  const int used = (length_of(p.prefix_lengths, p.prefix_lengths_64, g, p.P) + kT - 1) / kT;
+  if (used > 0) {
+    const int blk = flat / kT;
+    const bool pair = blk < 2 * p.pairs;
+    const Cuts cuts = pair ? p.cuts[0] : p.cuts[1];
+    const int rows = pair ? kT : p.part_rows[1], seg = pair ? gh * p.pairs + (blk >> 1) : gh;
+    const int first = range_of(cuts, seg * p.tiles_p), n = range_of(cuts, seg * p.tiles_p + used - 1) + 1 - first;
+    const float4* part = reinterpret_cast<const float4*>(pair ? p.part[0] : p.part[1]);
+    const float2* stat = pair ? p.stat[0] : p.stat[1];
+    const int r = live ? flat - blk * kT : 0;
 #pragma unroll 4
-    for (int j = 0; j < here; ++j) {
-      const float fj = __shfl_sync(0xffffffffu, f, j);
-      const float* sj = reinterpret_cast<const float*>(
-                            __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(src), j)) + lane * E;
-      float t[E];
-      if constexpr (E == 4) {
-        const float4 u = *reinterpret_cast<const float4*>(sj);
-        t[0] = u.x, t[1] = u.y, t[2] = u.z, t[3] = u.w;
-      } else {
-        const float2 u = *reinterpret_cast<const float2*>(sj);
-        t[0] = u.x, t[1] = u.y;
-      }
-#pragma unroll
-      for (int e = 0; e < E; ++e) o[e] += fj != 0.f ? fj * t[e] : 0.f;
+    for (int k = wp; k < n; k += Parts) {
+      const int64_t at = (pair ? 2 * (static_cast<int64_t>(first) + k + seg) + (blk & 1)
+                               : static_cast<int64_t>(first) + k + seg) * rows;
+      piece(part + at * (D / 4) + r, stat + at + r, rows);
     }
   }
-#pragma unroll
-  for (int e = 0; e < E; ++e) sO[warp][lane * E + e] = o[e];
-  if (lane == 0) sML[warp] = make_float2(M, L);
-  __syncthreads();
-  if (threadIdx.x < D / 2) {
-    float top = -INFINITY, total = 0.f, x0 = 0.f, x1 = 0.f;
-#pragma unroll
-    for (int w = 0; w < kJoinWarps; ++w) top = fmaxf(top, sML[w].x);
-#pragma unroll
-    for (int w = 0; w < kJoinWarps; ++w) {
-      const float f = sML[w].y > 0.f ? exp2f(sML[w].x - top) : 0.f;
-      total += f * sML[w].y;
-      x0 += f * sO[w][2 * threadIdx.x];
-      x1 += f * sO[w][2 * threadIdx.x + 1];
+  // pieces of the row's own keys
+  const int used2 = live ? (length_of(p.lengths, p.lengths_64, b, p.S) + kT - 1) / kT : 0;
+  if (used2 > 0) {
+    const int own = i * p.rep + hr, blk = own / kT, rows = p.part_rows[2];
+    const int seg = (b * p.Hk + hk) * p.own_blocks + blk;
+    const int first = range_of(p.cuts[2], seg * p.tiles_o);
+    const int n = range_of(p.cuts[2], seg * p.tiles_o + used2 - 1) + 1 - first;
+    for (int k = Parts - 1 - wp; k < n; k += Parts) {
+      const int64_t at = (static_cast<int64_t>(first) + k + seg) * rows;
+      const int r = own - blk * kT;
+      piece(reinterpret_cast<const float4*>(p.part[2]) + at * (D / 4) + r, p.stat[2] + at + r, rows);
     }
-    const float inv = total > 0.f ? 1.0f / total : 0.f;
-    reinterpret_cast<uint32_t*>(p.o)[row * (D / 2) + threadIdx.x] = pack2<T>(x0 * inv, x1 * inv);
+  }
+  if (wc == 0 && lane < 8) sML[wp][lane] = make_float2(M, L);
+  if (wp > 0) {
+#pragma unroll
+    for (int f = 0; f < F; ++f) sO[wp - 1][(lane >> 3) + 4 * (wc + kJoinCols * f)][lane & 7] = o[f];
+  }
+  __syncthreads();
+  if (wp > 0 || !live) return;
+  float top = M, total = 0.f, w[Parts];
+#pragma unroll
+  for (int q = 1; q < Parts; ++q) top = fmaxf(top, sML[q][lane & 7].x);
+#pragma unroll
+  for (int q = 0; q < Parts; ++q) {
+    const float2 ml = sML[q][lane & 7];
+    w[q] = ml.y > 0.f ? fast_exp2(ml.x - top) : 0.f;
+    total += w[q] * ml.y;
+  }
+  const float inv = total > 0.f ? 1.0f / total : 0.f;
+  T* out = reinterpret_cast<T*>(p.o) + ((static_cast<int64_t>(b) * p.Lq + i) * p.Hq + hk * p.rep + hr) * D;
+#pragma unroll
+  for (int f = 0; f < F; ++f) {
+    const int c4 = (lane >> 3) + 4 * (wc + kJoinCols * f);
+    float4 x = make_float4(w[0] * o[f].x, w[0] * o[f].y, w[0] * o[f].z, w[0] * o[f].w);
+#pragma unroll
+    for (int q = 1; q < Parts; ++q) {
+      const float4 t = sO[q - 1][c4][lane & 7];
+      x = make_float4(x.x + w[q] * t.x, x.y + w[q] * t.y, x.z + w[q] * t.z, x.w + w[q] * t.w);
+    }
+    *reinterpret_cast<uint2*>(out + 4 * c4) = make_uint2(pack2<T>(x.x * inv, x.y * inv), pack2<T>(x.z * inv, x.w * inv));
   }
 }
 
@@ -730,7 +740,14 @@ void launch(const CUtensorMap& pk, const CUtensorMap& pv, const CUtensorMap& k, 
   FYB_CUDA(cudaFuncSetAttribute(spa_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, spa_smem<D>()));
   spa_kernel<T, D><<<p.ctas, kSpaThreads, spa_smem<D>(), cur_stream()>>>(pk, pv, k, v, p);
   check_launch("shared_prefix_attention");
-  spa_join_kernel<T, D><<<p.B * p.Lq * p.Hq, kJoinWarps * 32, 0, cur_stream()>>>(p);
+  const int groups = p.G * p.Hk * ((p.rows_p + 7) / 8);
+  // pieces of a row, about: ranges that meet a prefix block and those of its own keys
+  const int segs = p.G * p.Hk * std::max(p.pairs, 1);
+  const int pieces = (p.pairs > 0 ? p.cuts[0].units : p.cuts[1].units) / segs + 2;
+  if (pieces > 8)
+    spa_join_kernel<T, D, 4><<<groups, kJoinCols * 4 * 32, 0, cur_stream()>>>(p);
+  else
+    spa_join_kernel<T, D, 2><<<groups, kJoinCols * 2 * 32, 0, cur_stream()>>>(p);
   check_launch("shared_prefix_attention (join)");
 }
 
@@ -771,15 +788,18 @@ at::Tensor shared_prefix_attention(const at::Tensor& q, const at::Tensor& pk, co
   p.tiles_p = (int)((P + kT - 1) / kT);
   p.tiles_o = (int)((S + kT - 1) / kT);
   const int64_t segs[3] = {G * Hk * p.pairs, G * Hk * p.odd, B * Hk * p.own_blocks};
+  int total[3];
   for (int c = 0; c < 3; ++c) {
     const int64_t tiles = segs[c] * (c == 2 ? p.tiles_o : p.tiles_p);
     FYB_CHECK(tiles < (1ll << 31), "shared_prefix_attention: more than 2^31 tiles");
-    p.total[c] = (int)tiles;
-    p.inv_total[c] = tiles > 0 ? 1.0 / (double)tiles : 0.0;
+    total[c] = (int)tiles;
   }
   p.ctas = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
-  for (int c = 0; c < 3; ++c) p.units[c] = std::min(p.total[c], c == 0 ? p.ctas : 2 * p.ctas);
-  p.shift = p.units[1] % (2 * p.ctas);
+  for (int c = 0; c < 3; ++c) {
+    const int units = std::min(total[c], c == 0 ? p.ctas : 2 * p.ctas);
+    p.cuts[c] = units > 0 ? Cuts{units, total[c] / units, total[c] % units} : Cuts{0, 1, 0};
+  }
+  p.shift = p.cuts[1].units % (2 * p.ctas);
   p.lengths = length_ptr(lengths, q, B, p.lengths_64);
   p.prefix_lengths = length_ptr(prefix_lengths, q, G, p.prefix_lengths_64);
   p.scale_log2 = (float)(scale * 1.4426950408889634);
@@ -791,8 +811,8 @@ at::Tensor shared_prefix_attention(const at::Tensor& q, const at::Tensor& pk, co
   p.part_rows[2] = std::min(p.rows_o, kT);
   int64_t rows[3], all = 0;
   for (int c = 0; c < 3; ++c) {
-    const int64_t slots = (p.units[c] + segs[c]) * (c == 0 ? 2 : 1);
-    rows[c] = p.total[c] > 0 ? slots * p.part_rows[c] : 0;
+    const int64_t slots = (p.cuts[c].units + segs[c]) * (c == 0 ? 2 : 1);
+    rows[c] = total[c] > 0 ? slots * p.part_rows[c] : 0;
     all += rows[c];
   }
   auto ws = at::empty({std::max<int64_t>(all, 1) * (D + 2)}, q.options().dtype(at::kFloat));
