@@ -338,16 +338,18 @@ __global__ void __launch_bounds__(kSpaThreads, 1)
     // descriptors: a tile's own bits plus its address and the K step's offset, both in units of 16 bytes
     const uint64_t desc_km = sw128_desc(0, 16, 1024), desc_mn = sw128_desc(0, kAtom, 1024);
     const uint32_t q16 = uniform(smem_u32(sQ) >> 4), kv16 = uniform(smem_u32(sKV) >> 4), tm = uniform(tmem);
+    auto meet_v = [&](const Product& v) -> bool {
+      if (!v.pending || v.follows) return true;
+      if (!wait(&bars->full[ring.slot], ring.phase, 711)) return false;
+      v_slot = ring.slot;
+      ring.step();
+      return true;
+    };
     auto issue_pv = [&](Product& v, int s) -> bool {
       if (!v.pending) return true;
       v.pending = false;
       if (!wait(&bars->p_full[s], v.pph, 710)) return false;
       v.pph ^= 1u;
-      if (!v.follows) {
-        if (!wait(&bars->full[ring.slot], ring.phase, 711)) return false;
-        v_slot = ring.slot;
-        ring.step();
-      }
       const int steps = (v.nv + 15) / 16;
       if (!v.follows && v.nv < steps * 16) {
         // a weight of zero times what lies behind the last key in use has to be zero (whole rows: no swizzle)
@@ -387,14 +389,19 @@ __global__ void __launch_bounds__(kSpaThreads, 1)
       const int s = st.turn;
       const Walk& x = st.w;
       // a stream that has ended must not hold its V tile while the other goes on (its product is the younger one)
-      if (!(ok = issue_pv(st.s, s))) break;
-      if (!st.live_other && st.s_other.pending) {
-        free_v();
-        if (!(ok = issue_pv(st.s_other, s ^ 1))) break;
-      }
       const bool follows = st.follows();
       const int nv = min(kT, x.len - x.t * kT);
       const bool last = x.t + 1 >= x.t1, frees = x.cls != 0 || follows;
+      // what was loaded ahead is waited for before the softmax, so that both products go out together; the scores' tile
+      // needs no slot that the product before it still holds
+      const bool flush = !st.live_other && st.s_other.pending;
+      if (!(ok = meet_v(st.s))) break;
+      if (flush) {
+        // a stream that has ended must not hold its V tile while the other goes on (its product is the younger one)
+        if (!(ok = issue_pv(st.s, s))) break;
+        free_v();
+        if (!(ok = meet_v(st.s_other) && issue_pv(st.s_other, s ^ 1))) break;
+      }
       if (!follows) {
         if (!(ok = wait(&bars->full[ring.slot], ring.phase, 712))) break;
         k_slot = ring.slot;
@@ -404,6 +411,7 @@ __global__ void __launch_bounds__(kSpaThreads, 1)
         if (!(ok = wait(&bars->q_full[s], st.s.qph, 713))) break;
         st.s.qph ^= 1u;
       }
+      if (!(ok = issue_pv(st.s, s))) break;
       const int u = uniform(k_slot | s << 4 | (frees ? 32 : 0) | (last ? 64 : 0) | (nv + 15) / 16 << 8);
       const int ks = u & 15, su = u >> 4 & 1;
       const uint32_t id = idesc_of<T>(0, false) | static_cast<uint32_t>(u >> 8) << 18;     // N = 16 x count
@@ -430,9 +438,9 @@ __global__ void __launch_bounds__(kSpaThreads, 1)
       st.s.first = last;
     }
     // the products left over: the stream that did not take the last step holds the older one
-    if (ok) ok = issue_pv(st.s_other, st.turn ^ 1);
+    if (ok) ok = meet_v(st.s_other) && issue_pv(st.s_other, st.turn ^ 1);
     free_v();
-    if (ok) ok = issue_pv(st.s, st.turn);
+    if (ok) ok = meet_v(st.s) && issue_pv(st.s, st.turn);
     free_v();
   } else if (warp < 4) {
     // ----------------------------------------------------------------------------------------------- query blocks
