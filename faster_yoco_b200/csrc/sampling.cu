@@ -4,15 +4,24 @@
 // the shortest prefix with at least p of the weight left and to w_i >= min_p; the token is the first kept index whose
 // running weight in index order passes u times the kept weight.
 //
-// No sort: every cut is a threshold (a value and how many of its ties, by index, are kept), found by a radix search
-// over the order-preserving 32-bit image of the logits, most significant digit first, with a histogram of counts
-// (top-k) or of weights (top-p) for each digit.
+// No sort of the vocabulary. A cluster of 1 to 8 CTAs has a row, each CTA a contiguous slice, each warp a contiguous
+// segment of it, so that running weights in index order are sums of segments. Passes over the row (the first from memory,
+// the others from L2):
+//   1  the largest logit, overall and of each thread
+//   2  the weight of each segment, where a filter needs the whole vocabulary's (top-p without top-k, or no filter)
+//   3  the candidates above a bound that no cut can pass: k-th largest of a CTA's thread maxima (k elements reach it);
+//      (1 - p) Z / V (the tail from the p-cut on weighs at least (1 - p) Z and has at most V elements); min_p. They are
+//      usually a few hundred: one CTA ranks them in shared memory, cuts and draws.
+//   Otherwise the cut is found by a radix search over the order-preserving 32-bit image of the logits, with histograms of
+//   counts (top-k) or weights (top-p) in steps of 11 bits, and the draw goes by segment sums.
 //
-// Tokens are decided by comparing sums over the whole vocabulary, so weights are evaluated in 64 bits and summed as
-// 64-bit integers (a fixed point that leaves room for V weights of at most 1): integer sums do not depend on the order
-// of the additions, so neither the token nor its log-probability depends on how the row is divided.
+// Tokens are decided by comparing sums over the whole vocabulary, so weights are evaluated to 2^-48 in 64 bits and
+// summed in 64 bits: histograms as integers in a fixed point that leaves room for V weights of 1, the rest in floating
+// point in a fixed order. Bound by the 64-bit exponential (11 operations at 60 a clock and SM) where every weight is
+// needed, else by reading the logits.
 #include <ATen/ATen.h>
 #include <c10/util/Optional.h>
+#include <cooperative_groups.h>
 #include <cuda_fp16.h>
 
 #include "common/host.h"
@@ -21,16 +30,21 @@
 namespace fyb {
 namespace {
 
+namespace cg = cooperative_groups;
+
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
+constexpr int kMaxCluster = 8;
+constexpr int kGranules = 8;        // pieces of a warp's segment whose weights are kept
+constexpr int kList = kThreads;     // candidates of the short list: one a thread
+constexpr int kBinBits = 11;        // of a radix step
 constexpr uint32_t kFull = 0xffffffffu;
-constexpr double kLog2e64 = 1.4426950408889634074;
-constexpr int64_t kNone = -1;
 
 struct SampleParams {
   const void* logits;
   int64_t ld;                // row stride (elements)
-  int64_t V;
+  int V;
+  int chunks;                // 8-element chunks of a CTA's slice
   const float* u;
   const float* temperature;  // per row, or null: temperature_all
   const void* top_k;         // per row (int32 or int64), or null
@@ -60,25 +74,85 @@ __device__ __forceinline__ float value_of(uint32_t k) {
   return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);
 }
 
-template <typename T>
-struct Row {
-  const T* x;
-  int64_t V;
+// w = 2^(t / 32) for t = 32 log2(e) (x - max) / T <= 0, by a table of 2^(j / 32) and a polynomial on |r| <= 1/2 (the table-driven
+// method of P. T. P. Tang, 1989): 2^(r / 32) = 1 + r (c1 + r (c2 + ...)), c_i = (ln 2 / 32)^i / i!; the remainder after r^5 is
+// below 2^-48. The table lies in the lanes of the warp (lane j: 2^(j / 32)) and is read by shuffles: all lanes call.
+struct Weight {
+  double top, scale, table;  // largest logit, 32 log2(e) / T, this lane's 2^(lane / 32)
+  float topf, scalef;
   uint32_t kmax;
-  double top, inv_t;   // largest logit, log2(e) / T
 
-  __device__ __forceinline__ uint32_t key(int64_t i) const { return key_of(to_float(x[i])); }
-  // weight of a candidate's image (> 0); exactly 1 for the largest
-  __device__ __forceinline__ double weight(uint32_t k) const {
-    if (k == kmax) return 1.0;
-    const double t = (static_cast<double>(value_of(k)) - top) * inv_t;
-    return t > -1000.0 ? exp2(t) : 0.0;    // NaN (0 * inf) also gives 0
+  __device__ __forceinline__ void init(uint32_t largest, float t) {
+    kmax = largest;
+    topf = value_of(largest);
+    top = static_cast<double>(topf);
+    scale = 46.166241308446828384 / static_cast<double>(t);
+    scalef = static_cast<float>(scale);
+  }
+  // weight of a logit; 0 for what is no candidate, exactly 1 for the largest
+  __device__ __forceinline__ double operator()(float x) const {
+    constexpr double kRound = 6755399441055744.0;        // 1.5 x 2^52: adding it rounds to an integer
+    constexpr double l = 0.021660849392498290;           // ln 2 / 32
+    // infinities, NaN and what is below 2^-1000 are told by a 32-bit estimate (NaN compares as false)
+    const bool some = fmaf(x, scalef, -topf * scalef) > -32000.0f;
+    const double d = some ? static_cast<double>(x) - top : 0.0;
+    const double z = fma(d, scale, kRound);
+    const double r = fma(d, scale, kRound - z);
+    const int n = __double2loint(z);
+    const int lo = __shfl_sync(kFull, __double2loint(table), n & 31);
+    const int hi = __shfl_sync(kFull, __double2hiint(table), n & 31);
+    double q = fma(r, l * l * l * l * l / 120, l * l * l * l / 24);
+    q = fma(q, r, l * l * l / 6);
+    q = fma(q, r, l * l / 2);
+    q = fma(q, r, l);
+    const double b = __hiloint2double(hi + ((n >> 5) << 20), lo);
+    const double w = fma(b * r, q, b);
+    return x == topf ? 1.0 : (some ? w : 0.0);
   }
 };
 
-__device__ __forceinline__ uint64_t fixed(double w, double unit) {
-  return static_cast<uint64_t>(__double2ll_rn(w * unit));
-}
+// Eight logits of a row: chunk c holds elements 8 c - off .. 8 c - off + 7, where off brings the row to a 16-byte boundary;
+// -inf outside the row.
+template <typename T>
+struct Row {
+  const T* x;
+  int V, off, chunks;
+
+  __device__ __forceinline__ Row(const SampleParams& p, int64_t n)
+      : x(reinterpret_cast<const T*>(p.logits) + n * p.ld), V(p.V) {
+    off = static_cast<int>((reinterpret_cast<uintptr_t>(x) & 15u) / sizeof(T));
+    chunks = (V + off + 7) / 8;
+  }
+  __device__ __forceinline__ int index(int c, int j) const { return 8 * c - off + j; }
+  __device__ __forceinline__ void load(int c, float (&v)[8]) const {
+    const int i = 8 * c - off;
+    if (c < chunks && i >= 0 && i + 8 <= V) {
+      if constexpr (sizeof(T) == 4) {
+        const float4 a = *reinterpret_cast<const float4*>(x + i), b = *reinterpret_cast<const float4*>(x + i + 4);
+        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+      } else {
+        const uint4 a = *reinterpret_cast<const uint4*>(x + i);
+        const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          float2 f;
+          if constexpr (std::is_same<T, __half>::value)
+            f = __half22float2(*reinterpret_cast<const __half2*>(&w[k]));
+          else
+            f = unpack_bf16(w[k]);
+          v[2 * k] = f.x;
+          v[2 * k + 1] = f.y;
+        }
+      }
+      return;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      v[j] = -INFINITY;
+      if (c < chunks && i + j >= 0 && i + j < V) v[j] = to_float(x[i + j]);
+    }
+  }
+};
 
 template <typename V>
 __device__ __forceinline__ V warp_sum(V v) {
@@ -86,219 +160,645 @@ __device__ __forceinline__ V warp_sum(V v) {
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
   return v;
 }
-
-// sum over the block, returned to every thread
-template <typename V>
-__device__ __forceinline__ V block_sum(V v, V* scratch) {
-  v = warp_sum(v);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
-  __syncthreads();
-  V s = 0;
-  for (int i = 0; i < kWarps; ++i) s += scratch[i];
-  return s;
+__device__ __forceinline__ uint64_t warp_max(uint64_t v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const uint64_t c = __shfl_xor_sync(kFull, v, o);
+    v = c > v ? c : v;
+  }
+  return v;
 }
 
 struct Cut {
   uint32_t key;         // images above are kept, those below are not
-  uint64_t ties;        // how many images equal to `key` are kept (the first ones by index)
+  uint32_t ties;        // how many images equal to `key` are kept (the first ones by index)
 };
 
-// Digit by digit search for the image where the running amount, from the largest image down, first reaches `target`:
-// amount = 1 for each candidate (kWeights false) or its fixed-point weight, over the candidates that `cut` keeps.
-// Returns the image; above: the amount of larger images; at: the number of candidates with it.
-template <typename T, bool kWeights>
-__device__ uint32_t radix_find(const Row<T>& row, const Cut& cut, double unit, double target, uint64_t* hist,
-                               uint64_t* scratch, uint64_t& above, uint64_t& at) {
-  uint32_t prefix = 0;
-  above = 0;
-  at = 0;
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    __syncthreads();
-    for (int i = threadIdx.x; i < 256; i += kThreads) hist[i] = 0;
-    __syncthreads();
-    for (int64_t i = threadIdx.x; i < row.V; i += kThreads) {
-      const uint32_t k = row.key(i);
-      if (k == 0 || k <= cut.key) continue;
-      if (shift < 24 && (k >> (shift + 8)) != (prefix >> (shift + 8))) continue;
-      const uint64_t a = kWeights ? fixed(row.weight(k), unit) : 1;
-      atomicAdd(reinterpret_cast<unsigned long long*>(&hist[(k >> shift) & 255u]), static_cast<unsigned long long>(a));
-    }
-    __syncthreads();
-    if (threadIdx.x == 0 && cut.ties > 0 && (shift == 24 || (cut.key >> (shift + 8)) == (prefix >> (shift + 8))))
-      hist[(cut.key >> shift) & 255u] += kWeights ? cut.ties * fixed(row.weight(cut.key), unit) : cut.ties;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      uint64_t run = above;
-      int d = 255, last = -1;
-      for (; d >= 0; --d) {
-        if (hist[d] == 0) continue;
-        last = d;
-        if (static_cast<double>(run + hist[d]) >= target) break;
-        run += hist[d];
-      }
-      if (d < 0) {               // rounding only: the smallest digit that occurs
-        d = last < 0 ? 0 : last;
-        run -= last < 0 ? 0 : hist[d];
-      }
-      scratch[0] = static_cast<uint64_t>(d);
-      scratch[1] = run;
-      scratch[2] = hist[d];
-    }
-    __syncthreads();
-    prefix |= static_cast<uint32_t>(scratch[0]) << shift;
-    above = scratch[1];
-    at = scratch[2];
-    __syncthreads();
-  }
-  return prefix;
-}
+struct Shared {
+  uint64_t warp_best[kWarps];
+  uint64_t best;                       // of this CTA: image << 32 | ~index
+  uint32_t bound;                      // of this CTA
+  double part[kWarps][kGranules];      // weight of each granule
+  double part_sum[kWarps];
+  double sum;                          // of this CTA
+  uint32_t count[kWarps];
+  uint32_t total_count;                // of this CTA (candidates, or ties)
+  uint32_t hist_lo[1 << kBinBits], hist_hi[1 << kBinBits];
+  uint64_t scan[kWarps];
+  uint64_t found[3];
+  // the short list, in the CTA that draws from it
+  uint32_t key[kList], idx[kList];
+  double w[kList];
+  uint32_t by_key[kList];              // list position by rank
+};
 
+// What the CTAs of a row know of one another goes through a field of Shared that each writes once before a cluster barrier
+// and that is written again only behind another one.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) sample_kernel(SampleParams p) {
-  __shared__ uint64_t hist[256];
-  __shared__ uint64_t scratch[2 * kWarps];
-  __shared__ uint64_t seg_w[kWarps], seg_t[kWarps];
-  const int64_t n = blockIdx.x;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+struct Sampler {
+  const SampleParams& p;
+  Shared& sh;
+  cg::cluster_group cluster;
   Row<T> row;
-  row.x = reinterpret_cast<const T*>(p.logits) + n * p.ld;
-  row.V = p.V;
+  Weight weight;
+  int rank, ctas, warp, lane;
+  int c0, c1, per, iters, step;        // this warp's chunks; chunks and iterations a warp, iterations of a granule
 
-  // largest image, lowest index
-  uint64_t best = 0;
-  for (int64_t i = threadIdx.x; i < p.V; i += kThreads) {
-    const uint64_t c = (static_cast<uint64_t>(row.key(i)) << 32) | static_cast<uint32_t>(~static_cast<uint32_t>(i));
-    best = c > best ? c : best;
+  __device__ __forceinline__ Sampler(const SampleParams& p_, Shared& s, int64_t n)
+      : p(p_), sh(s), cluster(cg::this_cluster()), row(p_, n) {
+    rank = cluster.block_rank();
+    ctas = cluster.num_blocks();
+    warp = threadIdx.x >> 5;
+    lane = threadIdx.x & 31;
+    per = (p.chunks + kWarps - 1) / kWarps;
+    iters = (per + 31) / 32;
+    step = (iters + kGranules - 1) / kGranules;
+    const int end = min((rank + 1) * p.chunks, row.chunks);
+    c0 = min(rank * p.chunks + warp * per, end);
+    c1 = min(c0 + per, end);
+    weight.table = exp2(lane / 32.0);
   }
+  __device__ __forceinline__ const Shared& of(int r) const {
+    return ctas == 1 ? sh : *cluster.map_shared_rank(&sh, r);
+  }
+  __device__ __forceinline__ void sync() {
+    if (ctas == 1)
+      __syncthreads();
+    else
+      cluster.sync();
+  }
+  // chunk of this lane at an iteration, or one outside the row
+  __device__ __forceinline__ int chunk(int it) const {
+    const int c = c0 + it * 32 + lane;
+    return c < c1 ? c : row.chunks;
+  }
+
+  // largest logit of the row (image << 32 | ~index); thread_key: this thread's largest image
+  __device__ __forceinline__ uint64_t largest(uint32_t& thread_key) {
+    float best = -INFINITY;
+    int at = 0;
+#pragma unroll 4
+    for (int it = 0; it < iters; ++it) {
+      float v[8];
+      const int c = chunk(it);
+      row.load(c, v);
+      float m = -INFINITY;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const uint64_t c = __shfl_xor_sync(kFull, best, o);
-    best = c > best ? c : best;
-  }
-  if (lane == 0) scratch[warp] = best;
-  __syncthreads();
-  for (int i = 0; i < kWarps; ++i) best = scratch[i] > best ? scratch[i] : best;
-  row.kmax = static_cast<uint32_t>(best >> 32);
-  const float t = p.temperature != nullptr ? p.temperature[n] : p.temperature_all;
-  if (row.kmax == 0 || !(t > 0.f)) {
-    if (threadIdx.x == 0) {
-      p.token[n] = row.kmax == 0 ? kNone : static_cast<int64_t>(~static_cast<uint32_t>(best));
-      if (p.logprob != nullptr) p.logprob[n] = row.kmax == 0 ? -INFINITY : 0.f;
+      for (int j = 0; j < 8; ++j) m = fmaxf(m, v[j]);      // drops NaN
+      if (m > best) {                                      // chunks come in index order
+        best = m;
+        at = c;
+      }
     }
-    return;
+    thread_key = key_of(best);
+    uint64_t mine = 0;
+    if (thread_key != 0) {
+      float v[8];
+      row.load(at, v);
+      int j = 7;
+#pragma unroll
+      for (int k = 7; k >= 0; --k)
+        if (v[k] == best) j = k;
+      mine = static_cast<uint64_t>(thread_key) << 32 | static_cast<uint32_t>(~static_cast<uint32_t>(row.index(at, j)));
+    }
+    mine = warp_max(mine);
+    if (lane == 0) sh.warp_best[warp] = mine;
+    __syncthreads();
+    uint64_t b = lane < kWarps ? sh.warp_best[lane] : 0;
+    b = warp_max(b);
+    if (ctas == 1) return b;
+    if (threadIdx.x == 0) sh.best = b;
+    cluster.sync();
+    b = lane < ctas ? of(lane).best : 0;
+    return warp_max(b);
   }
-  row.top = static_cast<double>(value_of(row.kmax));
-  row.inv_t = kLog2e64 / static_cast<double>(t);
 
-  int64_t k = p.top_k_all;
-  if (p.top_k != nullptr)
-    k = p.top_k_64 ? reinterpret_cast<const int64_t*>(p.top_k)[n] : reinterpret_cast<const int*>(p.top_k)[n];
-  const float tp = p.top_p != nullptr ? p.top_p[n] : p.top_p_all;
-  const float mp = p.min_p != nullptr ? p.min_p[n] : p.min_p_all;
+  // An image that at least k elements of the row reach: the k-th largest of a CTA's thread maxima (k <= kThreads), the
+  // largest of these over the CTAs. Bit by bit: the largest image that k threads reach.
+  __device__ __forceinline__ uint32_t bound_of_k(uint32_t thread_key, int k) {
+    uint32_t b = 0;
+    for (int bit = 31; bit >= 0; --bit) {
+      const uint32_t t = b | (1u << bit);
+      if (__syncthreads_count(thread_key >= t) >= k) b = t;
+    }
+    if (ctas == 1) return b;
+    if (threadIdx.x == 0) sh.bound = b;
+    cluster.sync();
+    b = lane < ctas ? of(lane).bound : 0;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) b = max(b, __shfl_xor_sync(kFull, b, o));
+    return b;
+  }
 
-  Cut cut{0u, 0};
-  uint64_t above, at;
-  if (k > 0 && k < p.V) {
-    const uint32_t key = radix_find<T, false>(row, cut, p.unit, static_cast<double>(k), hist, scratch, above, at);
-    if (key != 0) {
+  // whether an element is kept: by the cut (ties: the first by index; tie_rank counts those of this warp's segment met so
+  // far, all lanes call) and by min_p
+  struct Kept {
+    Cut cut;
+    double min_w;
+  };
+
+  // weight of what is kept among the eight logits of each lane, in index order within the lane; w[j] = 0 for the others
+  __device__ __forceinline__ double weigh(const float (&v)[8], const Kept& kept, uint32_t& tie_rank, double (&w)[8]) {
+    double s = 0.0;
+    uint32_t mine = 0, before = 0;
+    if (kept.cut.key != 0) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) mine += key_of(v[j]) == kept.cut.key ? 1u : 0u;
+      uint32_t inc = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t c = __shfl_up_sync(kFull, inc, o);
+        if (lane >= o) inc += c;
+      }
+      before = tie_rank + inc - mine;
+      tie_rank += __shfl_sync(kFull, inc, 31);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      w[j] = 0.0;
+      const uint32_t k = key_of(v[j]);
+      bool keep = k > kept.cut.key;
+      if (kept.cut.key != 0 && k == kept.cut.key) keep = before++ < kept.cut.ties;
+      if (kept.cut.key != 0 && !__any_sync(kFull, keep)) continue;
+      const double x = weight(v[j]);
+      if (keep && x >= kept.min_w) w[j] = x;
+      s += w[j];
+    }
+    return s;
+  }
+
+  // ties of the cut before this warp's segment
+  __device__ __forceinline__ uint32_t ties_before(const Cut& cut) {
+    if (cut.key == 0) return 0;
+    uint32_t n = 0;
+#pragma unroll 2
+    for (int it = 0; it < iters; ++it) {
+      float v[8];
+      row.load(chunk(it), v);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) n += key_of(v[j]) == cut.key ? 1u : 0u;
+    }
+    n = warp_sum(n);
+    if (lane == 0) sh.count[warp] = n;
+    __syncthreads();
+    uint32_t before = 0, all = 0;
+    for (int i = 0; i < kWarps; ++i) {
+      if (i < warp) before += sh.count[i];
+      all += sh.count[i];
+    }
+    if (ctas > 1) {
+      if (threadIdx.x == 0) sh.total_count = all;
+      cluster.sync();
+      for (int r = 0; r < rank; ++r) before += of(r).total_count;
+    }
+    return before;
+  }
+
+  // weight of every granule; returns the row's
+  __device__ __forceinline__ double sums(const Kept& kept, uint32_t ties0) {
+    uint32_t tie_rank = ties0;
+    for (int g = 0; g < kGranules; ++g) {
+      double s = 0.0;
+      for (int it = g * step; it < min((g + 1) * step, iters); ++it) {
+        float v[8];
+        double w[8];
+        row.load(chunk(it), v);
+        s += weigh(v, kept, tie_rank, w);
+      }
+      s = warp_sum(s);
+      if (lane == 0) sh.part[warp][g] = s;
+    }
+    __syncthreads();
+    if (lane == 0) {
+      double s = 0.0;
+      for (int g = 0; g < kGranules; ++g) s += sh.part[warp][g];
+      sh.part_sum[warp] = s;
+    }
+    __syncthreads();
+    double s = 0.0;
+    for (int i = 0; i < kWarps; ++i) s += sh.part_sum[i];
+    if (ctas == 1) return s;
+    if (threadIdx.x == 0) sh.sum = s;
+    cluster.sync();
+    s = 0.0;
+    for (int r = 0; r < ctas; ++r) s += of(r).sum;
+    return s;
+  }
+
+  // first of n parts whose running sum (from `before`) passes r, the last with any weight if rounding hides it
+  template <typename F>
+  __device__ __forceinline__ int pass(int n, F part, double r, double& before) {
+    int last = 0;
+    double at_last = before;
+    for (int i = 0; i < n; ++i) {
+      const double s = part(i);
+      if (s > 0.0) {
+        last = i;
+        at_last = before;
+      }
+      if (before + s > r) return i;
+      before += s;
+    }
+    before = at_last;
+    return last;
+  }
+
+  // draws by the granules' weights (sums() of the same `kept` came before)
+  __device__ __forceinline__ void draw(int64_t n, const Kept& kept, uint32_t ties0, double total) {
+    const double r = fmin(fmax(static_cast<double>(p.u[n]), 0.0), 1.0 - 0x1p-24) * total;
+    double before = 0.0;
+    if (ctas > 1 && pass(ctas, [&](int i) { return of(i).sum; }, r, before) != rank) return;
+    if (pass(kWarps, [&](int i) { return sh.part_sum[i]; }, r, before) != warp) return;
+    const int g = pass(kGranules, [&](int i) { return sh.part[warp][i]; }, r, before);
+    uint32_t tie_rank = ties0;
+    float v[8];
+    double w[8];
+    if (kept.cut.key != 0)                       // ties of the granules before
+      for (int it = 0; it < g * step; ++it) {
+        row.load(chunk(it), v);
+        uint32_t t = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) t += key_of(v[j]) == kept.cut.key ? 1u : 0u;
+        tie_rank += warp_sum(t);
+      }
+    int found = -1;
+    double found_w = 0.0;
+    for (int it = g * step; it < min((g + 1) * step, iters); ++it) {
+      row.load(chunk(it), v);
+      const double mine = weigh(v, kept, tie_rank, w);
+      double inc = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const double c = __shfl_up_sync(kFull, inc, o);
+        if (lane >= o) inc += c;
+      }
+      const uint32_t hit = __ballot_sync(kFull, before + inc > r && mine > 0.0);
+      const uint32_t some = __ballot_sync(kFull, mine > 0.0);
+      if (some != 0) {
+        // the first lane that passes r; none yet: the last one with weight so far
+        const int l = hit != 0 ? __ffs(hit) - 1 : 31 - __clz(some);
+        const double base = before + __shfl_sync(kFull, inc - mine, l);
+        int at = -1;
+        double at_w = 0.0;
+        if (lane == l) {
+          double run = base;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const bool open = at < 0 || run <= r;
+            run += w[j];
+            if (w[j] > 0.0 && open) {
+              at = row.index(chunk(it), j);
+              at_w = w[j];
+            }
+          }
+        }
+        found = __shfl_sync(kFull, at, l);
+        found_w = __shfl_sync(kFull, at_w, l);
+      }
+      if (hit != 0) break;
+      before += __shfl_sync(kFull, inc, 31);
+    }
+    if (lane == 0) write(n, found, found_w, total);
+  }
+
+  __device__ __forceinline__ void write(int64_t n, int index, double w, double total) const {
+    p.token[n] = index;
+    if (p.logprob != nullptr) p.logprob[n] = static_cast<float>(log(w / total));
+  }
+
+  // Candidates of image >= bound, in index order in the first CTA's list; returns how many there are (more than kList:
+  // the list is not written)
+  __device__ __forceinline__ uint32_t gather(uint32_t bound, uint32_t thread_key) {
+    const bool has = thread_key >= bound;
+    const bool any = __any_sync(kFull, has);
+    uint32_t n = 0;
+    if (any) {
+#pragma unroll 2
+      for (int it = 0; it < iters; ++it) {
+        float v[8];
+        row.load(has ? chunk(it) : row.chunks, v);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) n += key_of(v[j]) >= bound ? 1u : 0u;
+      }
+      n = warp_sum(n);
+    }
+    if (lane == 0) sh.count[warp] = n;
+    __syncthreads();
+    uint32_t before = 0, all = 0;
+    for (int i = 0; i < kWarps; ++i) {
+      if (i < warp) before += sh.count[i];
+      all += sh.count[i];
+    }
+    if (ctas > 1) {
+      if (threadIdx.x == 0) sh.total_count = all;
+      cluster.sync();
+      all = 0;
+      for (int r = 0; r < ctas; ++r) {
+        if (r < rank) before += of(r).total_count;
+        all += of(r).total_count;
+      }
+    }
+    if (all > kList) return all;
+    if (any && n > 0) {
+      Shared& to = ctas == 1 ? sh : *cluster.map_shared_rank(&sh, 0);
+      for (int it = 0; it < iters; ++it) {
+        float v[8];
+        row.load(has ? chunk(it) : row.chunks, v);
+        uint32_t mine = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) mine += key_of(v[j]) >= bound ? 1u : 0u;
+        if (!__any_sync(kFull, mine != 0)) continue;
+        uint32_t inc = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const uint32_t c = __shfl_up_sync(kFull, inc, o);
+          if (lane >= o) inc += c;
+        }
+        uint32_t at = before + inc - mine;
+        before += __shfl_sync(kFull, inc, 31);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const uint32_t k = key_of(v[j]);
+          if (k >= bound) {
+            to.key[at] = k;
+            to.idx[at] = static_cast<uint32_t>(row.index(chunk(it), j));
+            ++at;
+          }
+        }
+      }
+    }
+    sync();
+    return all;
+  }
+
+  // inclusive sum over the threads of the block before and with this one, in a fixed order
+  template <typename V>
+  __device__ __forceinline__ V block_scan(V v, V* scratch) {
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const V c = __shfl_up_sync(kFull, v, o);
+      if (lane >= o) v += c;
+    }
+    __syncthreads();
+    if (lane == 31) scratch[warp] = v;
+    __syncthreads();
+    V before = 0;
+    for (int i = 0; i < warp; ++i) before += scratch[i];
+    return before + v;
+  }
+
+  // Cuts and draws from the list of n candidates, which holds everything that can be kept. z: weight of what top_p is a
+  // share of, or 0 where that is the first k candidates.
+  __device__ __forceinline__ void draw_list(int64_t n_row, int n, int k, float top_p, double min_w, double z) {
+    const int t = threadIdx.x;
+    const bool have = t < n;
+    const uint32_t key = have ? sh.key[t] : 0u;
+    const double w = weight(have ? value_of(key) : -INFINITY);
+    // rank in descending order; the list is in index order, so ties are won by the earlier position
+    int rank_k = 0;
+#pragma unroll 8
+    for (int j = 0; j < n; ++j) {
+      const uint32_t o = sh.key[j];
+      rank_k += (o > key || (o == key && j < t)) ? 1 : 0;
+    }
+    if (have) {
+      sh.by_key[rank_k] = static_cast<uint32_t>(t);
+      sh.w[t] = w;
+    }
+    __syncthreads();
+    double* scratch = sh.part_sum;
+    // in the order of ranks: thread t looks at the candidate of rank t
+    const int first = k > 0 ? min(k, n) : n;
+    const int who = have ? static_cast<int>(sh.by_key[t]) : 0;
+    const double wr = t < first ? sh.w[who] : 0.0;
+    const double inc = block_scan(wr, scratch);
+    __syncthreads();
+    if (t == kThreads - 1) sh.sum = inc;
+    __syncthreads();
+    const double share = static_cast<double>(top_p) * (z > 0.0 ? z : sh.sum);
+    bool keep = t < first && (t == 0 || top_p >= 1.f || inc - wr < share);
+    keep = keep && wr >= min_w;
+    __syncthreads();
+    if (have && !keep) sh.w[who] = 0.0;
+    __syncthreads();
+    // in index order
+    const double wi = have ? sh.w[t] : 0.0;
+    const double run = block_scan(wi, scratch);
+    __syncthreads();
+    if (t == kThreads - 1) sh.sum = run;
+    __syncthreads();
+    const double total = sh.sum;
+    const double r = fmin(fmax(static_cast<double>(p.u[n_row]), 0.0), 1.0 - 0x1p-24) * total;
+    // first with run > r; rounding cannot hide the last one, whose running sum is `total` itself
+    const bool hit = wi > 0.0 && run > r;
+    const uint32_t m = __ballot_sync(kFull, hit);
+    if (lane == 0) sh.count[warp] = m;
+    __syncthreads();
+    if (t == 0) {
+      for (int i = 0; i < kWarps; ++i) {
+        if (sh.count[i] == 0) continue;
+        const int at = 32 * i + __ffs(sh.count[i]) - 1;
+        write(n_row, static_cast<int>(sh.idx[at]), sh.w[at], total);
+        break;
+      }
+    }
+  }
+
+  __device__ __forceinline__ uint64_t fixed(double w) const { return static_cast<uint64_t>(__double2ll_rn(w * p.unit)); }
+
+  // The image at which the amount of larger and equal images first reaches `target`: 1 for each candidate that the cut
+  // keeps, or its fixed-point weight. Steps of kBinBits over the images from `low` (> 0) up, which hold the answer.
+  // above: the amount of larger images; at: the amount of that image.
+  template <bool kWeights>
+  __device__ uint32_t radix_find(const Cut& cut, uint32_t low, double target, uint64_t& above, uint64_t& at) {
+    uint32_t base = low;
+    int bits = 32 - __clz(weight.kmax - low);
+    above = 0;
+    at = 0;
+    do {
+      const int s = max(bits - kBinBits, 0);
+      const int bins = 1 << (bits - s);
+      __syncthreads();
+      for (int i = threadIdx.x; i < bins; i += kThreads) sh.hist_lo[i] = sh.hist_hi[i] = 0;
+      __syncthreads();
+      auto add = [&](uint32_t bin, uint64_t a) {
+        const uint32_t lo = static_cast<uint32_t>(a);
+        uint32_t hi = static_cast<uint32_t>(a >> 32);
+        const uint32_t old = atomicAdd(&sh.hist_lo[bin], lo);
+        hi += old + lo < old ? 1u : 0u;
+        if (hi != 0) atomicAdd(&sh.hist_hi[bin], hi);
+      };
+      for (int it = 0; it < iters; ++it) {
+        float v[8];
+        row.load(chunk(it), v);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const uint32_t k = key_of(v[j]);
+          const uint64_t span = static_cast<uint64_t>(k - base) >> bits;       // bits may be 32
+          const bool in = k > cut.key && k >= base && span == 0;
+          if (!__any_sync(kFull, in)) continue;
+          const uint64_t a = kWeights ? fixed(weight(v[j])) : 1;
+          if (in) add((k - base) >> s, a);
+        }
+      }
+      const double wt = weight(cut.key != 0 ? value_of(cut.key) : -INFINITY);
+      if (rank == 0 && threadIdx.x == 0 && cut.ties > 0 && cut.key >= base &&
+          (static_cast<uint64_t>(cut.key - base) >> bits) == 0)
+        add((cut.key - base) >> s, kWeights ? cut.ties * fixed(wt) : cut.ties);
+      sync();
+      // thread t adds up four bins, from the top; sums over the CTAs, the same in each
+      constexpr int kPer = (1 << kBinBits) / kThreads;
+      uint64_t h[kPer], mine = 0;
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) {
+        const int bin = bins - 1 - (static_cast<int>(threadIdx.x) * kPer + j);
+        h[j] = 0;
+        if (bin >= 0)
+          for (int r = 0; r < ctas; ++r)
+            h[j] += static_cast<uint64_t>(of(r).hist_hi[bin]) << 32 | of(r).hist_lo[bin];
+        mine += h[j];
+      }
+      const uint64_t inc = block_scan(mine, sh.scan);
+      if (threadIdx.x == 0) sh.found[0] = ~0ull;
+      __syncthreads();
+      // the first thread whose sum reaches the target; the last with any amount if rounding hides it
+      const bool reach = mine > 0 && static_cast<double>(above + inc) >= target &&
+                         !(static_cast<double>(above + inc - mine) >= target);
+      if (reach || (mine > 0 && static_cast<double>(above + inc) < target)) {
+        const uint64_t order = (reach ? 0ull : 1ull << 32) | (reach ? threadIdx.x : kThreads - threadIdx.x);
+        atomicMin(reinterpret_cast<unsigned long long*>(&sh.found[0]), static_cast<unsigned long long>(order));
+      }
+      __syncthreads();
+      const uint64_t order = sh.found[0];
+      const uint32_t winner = (order >> 32) == 0 ? static_cast<uint32_t>(order)
+                                                 : kThreads - static_cast<uint32_t>(order & 0xffffffffu);
+      if (threadIdx.x == winner) {
+        uint64_t run = above + inc - mine, here = 0, before = run;
+        int bin = 0;
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) {
+          const int b = bins - 1 - (static_cast<int>(threadIdx.x) * kPer + j);
+          if (h[j] > 0 && (here == 0 || static_cast<double>(run) < target)) {
+            bin = b;
+            here = h[j];
+            before = run;
+          }
+          run += h[j];
+        }
+        sh.found[1] = before;
+        sh.found[2] = here;
+        sh.scan[0] = static_cast<uint64_t>(bin);
+      }
+      __syncthreads();
+      base += static_cast<uint32_t>(sh.scan[0]) << s;
+      above = sh.found[1];
+      at = sh.found[2];
+      bits = s;
+      sync();
+    } while (bits > 0);
+    return base;
+  }
+
+  __device__ __forceinline__ void run(int64_t n) {
+    uint32_t thread_key;
+    const uint64_t best = largest(thread_key);
+    const float t = p.temperature != nullptr ? p.temperature[n] : p.temperature_all;
+    const uint32_t kmax = static_cast<uint32_t>(best >> 32);
+    const float mp = p.min_p != nullptr ? p.min_p[n] : p.min_p_all;
+    if (kmax == 0 || !(t > 0.f) || !(mp <= 1.f)) {         // min_p above 1 leaves the largest alone
+      if (rank == 0 && threadIdx.x == 0) {
+        p.token[n] = kmax == 0 ? -1 : static_cast<int64_t>(~static_cast<uint32_t>(best));
+        if (p.logprob != nullptr) p.logprob[n] = kmax == 0 ? -INFINITY : 0.f;
+      }
+      return;
+    }
+    weight.init(kmax, t);
+    int64_t k64 = p.top_k_all;
+    if (p.top_k != nullptr)
+      k64 = p.top_k_64 ? reinterpret_cast<const int64_t*>(p.top_k)[n] : reinterpret_cast<const int*>(p.top_k)[n];
+    const int k = k64 > 0 && k64 < p.V ? static_cast<int>(k64) : 0;
+    const float tp = p.top_p != nullptr ? p.top_p[n] : p.top_p_all;
+    const bool by_p = !(tp >= 1.f);
+    const double share = by_p ? fmax(static_cast<double>(tp), 0.0) : 1.0;
+    const double min_w = mp > 0.f ? static_cast<double>(mp) : 0.0;
+
+    // images from `low` up hold everything that is kept; 1 is below all candidates
+    uint32_t low = 1;
+    double z = 0.0;
+    Kept all{Cut{0, 0}, 0.0};
+    if (k > 0) {
+      if (k <= kThreads) low = max(bound_of_k(thread_key, k), 1u);
+    } else if (by_p) {
+      z = sums(all, 0);
+      low = bound_of_weight((1.0 - share) * z / p.V);
+    }
+    if (min_w > 0.0 && !(k > 0 && by_p)) low = max(low, bound_of_weight(min_w));
+    if (low > 1 || p.V <= kList) {
+      const uint32_t c = gather(low, thread_key);
+      if (c <= kList) {
+        if (rank == 0) draw_list(n, static_cast<int>(c), k, by_p ? static_cast<float>(share) : 1.f, min_w, z);
+        return;
+      }
+    }
+    Cut cut{0, 0};
+    uint64_t above, at;
+    if (k > 0) {
+      const uint32_t key = radix_find<false>(cut, 1, static_cast<double>(k), above, at);
       const uint64_t left = static_cast<uint64_t>(k) - min(above, static_cast<uint64_t>(k));
-      cut = Cut{key, left < at ? left : at};
+      cut = Cut{key, static_cast<uint32_t>(min(left, at))};
     }
-  }
-  if (!(tp >= 1.f)) {
-    uint64_t part = 0;
-    for (int64_t i = threadIdx.x; i < p.V; i += kThreads) {
-      const uint32_t key = row.key(i);
-      if (key > cut.key) part += fixed(row.weight(key), p.unit);
-    }
-    uint64_t all = block_sum(part, scratch);
-    if (cut.ties > 0) all += cut.ties * fixed(row.weight(cut.key), p.unit);
-    const double target = fmax(static_cast<double>(tp), 0.0) * static_cast<double>(all);
-    const uint32_t key = radix_find<T, true>(row, cut, p.unit, target, hist, scratch, above, at);
-    const uint64_t w = fixed(row.weight(key), p.unit);
-    uint64_t ties = ~0ull;
-    if (w > 0) {
-      const uint64_t have = at / w;
-      ties = 1;
-      if (target > static_cast<double>(above)) {
-        // smallest count with above + count * w >= target, from a quotient that may be off by one
+    if (by_p) {
+      // shares of fixed-point sums, so that the search and its target agree
+      uint64_t sum = 0;
+      for (int it = 0; it < iters; ++it) {
+        float v[8];
+        row.load(chunk(it), v);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const uint64_t a = fixed(weight(v[j]));
+          sum += key_of(v[j]) > cut.key ? a : 0;
+        }
+      }
+      const double wt = weight(cut.key != 0 ? value_of(cut.key) : -INFINITY);
+      sum = block_scan(sum, sh.scan);
+      __syncthreads();
+      if (threadIdx.x == kThreads - 1) sh.best = sum;
+      sync();
+      sum = cut.ties * fixed(wt);
+      for (int r = 0; r < ctas; ++r) sum += of(r).best;
+      const double target = fmax(share * static_cast<double>(sum), 1.0);     // the largest is always kept
+      const uint32_t key = radix_find<true>(cut, cut.key != 0 ? cut.key : 1, target, above, at);
+      const uint64_t w = fixed(weight(value_of(key)));
+      uint64_t ties = 1;
+      if (w > 0 && target > static_cast<double>(above)) {
+        // smallest count with above + count w >= target, from a quotient that may be off by one
+        const uint64_t have = at / w;
         ties = static_cast<uint64_t>((target - static_cast<double>(above)) / static_cast<double>(w));
         ties = ties > 1 ? ties - 1 : 1;
         while (ties < have && static_cast<double>(above + ties * w) < target) ++ties;
       }
+      if (key == cut.key && cut.ties < ties) ties = cut.ties;
+      cut = Cut{key, static_cast<uint32_t>(min(ties, static_cast<uint64_t>(0xffffffffu)))};
     }
-    if (key == cut.key && cut.ties < ties) ties = cut.ties;
-    cut = Cut{key, ties};
+    const Kept kept{cut, min_w};
+    const uint32_t ties0 = ties_before(cut);
+    draw(n, kept, ties0, sums(kept, ties0));
   }
 
-  // kept weight by segment: each warp owns a contiguous piece of the row
-  const int64_t seg = (p.V + kThreads - 1) / kThreads * 32;
-  const int64_t s0 = min(seg * warp, p.V), s1 = min(s0 + seg, p.V);
-  uint64_t ties = 0;
-  for (int64_t i = s0 + lane; i < s1; i += 32) ties += row.key(i) == cut.key ? 1 : 0;
-  ties = warp_sum(ties);
-  __syncthreads();
-  if (lane == 0) seg_t[warp] = ties;
-  __syncthreads();
-  uint64_t tie0 = 0;
-  for (int i = 0; i < warp; ++i) tie0 += seg_t[i];
-  const double floor_w = static_cast<double>(mp);
-  auto kept = [&](int64_t i, uint64_t& tie_run, double& w) -> bool {   // all lanes of the warp call it
-    const uint32_t key = i < s1 ? row.key(i) : 0u;
-    const bool tie = key != 0 && key == cut.key;
-    const uint32_t m = __ballot_sync(kFull, tie);
-    const uint64_t rank = tie_run + __popc(m & ((1u << lane) - 1u));
-    tie_run += __popc(m);
-    bool keep = key > cut.key || (tie && rank < cut.ties);
-    w = keep ? row.weight(key) : 0.0;
-    return keep && (w >= floor_w || key == row.kmax);
-  };
-  // u = 0 asks for the first index with any weight at all: there a weight counts at least one unit
-  const double u01 = fmin(fmax(static_cast<double>(p.u[n]), 0.0), 1.0 - 0x1p-24);
-  auto units = [&](double w) -> uint64_t {
-    const uint64_t f = fixed(w, p.unit);
-    return (u01 == 0.0 && f == 0 && w > 0.0) ? 1 : f;
-  };
-  uint64_t mine = 0, run_t = tie0;
-  for (int64_t i = s0 + lane; i - lane < s1; i += 32) {
-    double w;
-    if (kept(i, run_t, w)) mine += units(w);
+  // an image that every weight >= w reaches (rounded down by more than its own and the weights' rounding)
+  __device__ __forceinline__ uint32_t bound_of_weight(double w) {
+    const double x = weight.top + log2(w) * 32.0 / weight.scale;           // w = 0: -inf
+    const float f = __double2float_rd(x - 1e-9 * (1.0 + fabs(x)));
+    return max(key_of(f), 1u);                                             // NaN, -inf: all candidates
   }
-  mine = warp_sum(mine);
-  if (lane == 0) seg_w[warp] = mine;
-  __syncthreads();
-  uint64_t total = 0, before = 0;
-  for (int i = 0; i < kWarps; ++i) {
-    if (i < warp) before += seg_w[i];
-    total += seg_w[i];
-  }
-  const double r = u01 * static_cast<double>(total);
-  if (static_cast<double>(before) > r || !(static_cast<double>(before + mine) > r)) return;
-  // this warp's segment holds the token
-  run_t = tie0;
-  for (int64_t i = s0 + lane; i - lane < s1; i += 32) {
-    double w;
-    const bool keep = kept(i, run_t, w);
-    uint64_t run = keep ? units(w) : 0;
-    const uint64_t own_w = run;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const uint64_t c = __shfl_up_sync(kFull, run, o);
-      if (lane >= o) run += c;
-    }
-    const bool hit = own_w > 0 && static_cast<double>(before + run) > r;
-    const uint32_t m = __ballot_sync(kFull, hit);
-    if (m != 0) {
-      if (lane == __ffs(m) - 1) {
-        p.token[n] = i;
-        if (p.logprob != nullptr)
-          p.logprob[n] = static_cast<float>(log(w) - log(static_cast<double>(total) / p.unit));
-      }
-      return;
-    }
-    before += __shfl_sync(kFull, run, 31);
-  }
+};
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_constant__ SampleParams p) {
+  __shared__ Shared sh;
+  Sampler<T> s(p, sh, blockIdx.x / cg::this_cluster().num_blocks());
+  s.run(blockIdx.x / cg::this_cluster().num_blocks());
+  s.sync();                            // a CTA's shared memory outlives the readers in its cluster
 }
 
 const void* row_param(const c10::optional<at::Tensor>& t, const at::Tensor& logits, at::ScalarType type,
@@ -308,6 +808,22 @@ const void* row_param(const c10::optional<at::Tensor>& t, const at::Tensor& logi
                 t->numel() == logits.size(0),
             std::string("sample: ") + name);
   return t->data_ptr();
+}
+
+template <typename T>
+void launch(const SampleParams& p, int64_t rows, int ctas) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(rows * ctas));
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = cur_stream();
+  cudaLaunchAttribute a[1];
+  a[0].id = cudaLaunchAttributeClusterDimension;
+  a[0].val.clusterDim.x = ctas;
+  a[0].val.clusterDim.y = a[0].val.clusterDim.z = 1;
+  cfg.attrs = a;
+  cfg.numAttrs = 1;
+  FYB_CUDA(cudaLaunchKernelEx(&cfg, sample_kernel<T>, p));
+  check_launch("sample");
 }
 
 }  // namespace
@@ -321,12 +837,15 @@ std::vector<at::Tensor> sample(const at::Tensor& logits, const at::Tensor& u,
   FYB_CHECK(logits.is_cuda() && logits.dim() == 2 && (logits.stride(1) == 1 || logits.size(1) == 1),
             "sample: logits [N, V] with a contiguous last dim expected");
   const int64_t N = logits.size(0), V = logits.size(1);
-  FYB_CHECK(V >= 1 && V < (1ll << 31) && N < (1ll << 31), "sample: sizes");
+  FYB_CHECK(V >= 1 && V < (1ll << 30) && N < (1ll << 27), "sample: sizes");
+  FYB_CHECK(logits.scalar_type() == at::kBFloat16 || logits.scalar_type() == at::kHalf ||
+                logits.scalar_type() == at::kFloat,
+            "sample: bf16, fp16 or fp32 logits expected");
   c10::cuda::CUDAGuard guard(logits.device());
   SampleParams p{};
   p.logits = logits.data_ptr();
   p.ld = logits.stride(0);
-  p.V = V;
+  p.V = static_cast<int>(V);
   FYB_CHECK(u.device() == logits.device() && u.scalar_type() == at::kFloat && u.is_contiguous() && u.numel() == N,
             "sample: u");
   p.u = u.data_ptr<float>();
@@ -348,15 +867,18 @@ std::vector<at::Tensor> sample(const at::Tensor& logits, const at::Tensor& u,
   p.token = token.data_ptr<int64_t>();
   p.logprob = want_logprob ? logprob.data_ptr<float>() : nullptr;
   if (N > 0) {
+    // CTAs a row: as many as two an SM allow, up to 8, while a thread still has a chunk of its own
+    const int64_t chunks = (V + 7 + 7) / 8;      // a row may start anywhere in its first chunk
+    const int sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
+    int ctas = 1;
+    while (ctas < kMaxCluster && N * ctas * 2 <= 2 * sms && chunks >= ctas * 2 * kThreads) ctas *= 2;
+    p.chunks = static_cast<int>((chunks + ctas - 1) / ctas);
     if (logits.scalar_type() == at::kBFloat16)
-      sample_kernel<__nv_bfloat16><<<N, kThreads, 0, cur_stream()>>>(p);
+      launch<__nv_bfloat16>(p, N, ctas);
     else if (logits.scalar_type() == at::kHalf)
-      sample_kernel<__half><<<N, kThreads, 0, cur_stream()>>>(p);
-    else if (logits.scalar_type() == at::kFloat)
-      sample_kernel<float><<<N, kThreads, 0, cur_stream()>>>(p);
+      launch<__half>(p, N, ctas);
     else
-      FYB_CHECK(false, "sample: bf16, fp16 or fp32 logits expected");
-    check_launch("sample");
+      launch<float>(p, N, ctas);
   }
   return {token, logprob};
 }
