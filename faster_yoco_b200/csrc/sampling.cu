@@ -78,8 +78,8 @@ __device__ __forceinline__ float value_of(uint32_t k) {
 // method of P. T. P. Tang, 1989): 2^(r / 32) = 1 + r (c1 + r (c2 + ...)), c_i = (ln 2 / 32)^i / i!; the remainder after r^5 is
 // below 2^-48. The table lies in the lanes of the warp (lane j: 2^(j / 32)) and is read by shuffles: all lanes call.
 struct Weight {
-  double top, scale, table;  // largest logit, 32 log2(e) / T, this lane's 2^(lane / 32)
-  float topf, scalef;
+  double top, scale, table;  // largest logit (finite), 32 log2(e) / T, this lane's 2^(lane / 32)
+  float topf, scalef, offset;  // in 32 bits; estimate of t: x scalef + offset
   uint32_t kmax;
 
   __device__ __forceinline__ void init(uint32_t largest, float t) {
@@ -88,26 +88,30 @@ struct Weight {
     top = static_cast<double>(topf);
     scale = 46.166241308446828384 / static_cast<double>(t);
     scalef = static_cast<float>(scale);
+    offset = -topf * scalef;
   }
-  // weight of a logit; 0 for what is no candidate, exactly 1 for the largest
-  __device__ __forceinline__ double operator()(float x) const {
+  // whether a logit has a weight: not -inf or NaN (the estimate is NaN, which compares as false), not below 2^-1000
+  __device__ __forceinline__ bool some(float x) const { return fmaf(x, scalef, offset) > -32000.0f || x == topf; }
+  // weight of a logit that has one, exactly 1 for the largest; anything for others
+  __device__ __forceinline__ double value(float x) const {
     constexpr double kRound = 6755399441055744.0;        // 1.5 x 2^52: adding it rounds to an integer
     constexpr double l = 0.021660849392498290;           // ln 2 / 32
-    // infinities, NaN and what is below 2^-1000 are told by a 32-bit estimate (NaN compares as false)
-    const bool some = fmaf(x, scalef, -topf * scalef) > -32000.0f;
-    const double d = some ? static_cast<double>(x) - top : 0.0;
+    const double d = static_cast<double>(x) - top;
     const double z = fma(d, scale, kRound);
     const double r = fma(d, scale, kRound - z);
     const int n = __double2loint(z);
-    const int lo = __shfl_sync(kFull, __double2loint(table), n & 31);
-    const int hi = __shfl_sync(kFull, __double2hiint(table), n & 31);
+    const int lo = __shfl_sync(kFull, __double2loint(table), n);           // (of the index the low five bits count)
+    const int hi = __shfl_sync(kFull, __double2hiint(table), n);
     double q = fma(r, l * l * l * l * l / 120, l * l * l * l / 24);
     q = fma(q, r, l * l * l / 6);
     q = fma(q, r, l * l / 2);
     q = fma(q, r, l);
-    const double b = __hiloint2double(hi + ((n >> 5) << 20), lo);
-    const double w = fma(b * r, q, b);
-    return x == topf ? 1.0 : (some ? w : 0.0);
+    const double b = __hiloint2double(hi + ((n << 15) & 0xfff00000), lo);
+    return fma(b * r, q, b);
+  }
+  __device__ __forceinline__ double operator()(float x) const {
+    const double w = value(x);
+    return some(x) ? w : 0.0;
   }
 };
 
@@ -117,6 +121,7 @@ template <typename T>
 struct Row {
   const T* x;
   int V, off, chunks;
+  bool only_inf = false;     // the largest logit is +inf: these count as 0, all others as -inf
 
   __device__ __forceinline__ Row(const SampleParams& p, int64_t n)
       : x(reinterpret_cast<const T*>(p.logits) + n * p.ld), V(p.V) {
@@ -124,9 +129,10 @@ struct Row {
     chunks = (V + off + 7) / 8;
   }
   __device__ __forceinline__ int index(int c, int j) const { return 8 * c - off + j; }
+  __device__ __forceinline__ bool whole(int c) const { return c < chunks && 8 * c >= off && 8 * c - off + 8 <= V; }
   __device__ __forceinline__ void load(int c, float (&v)[8]) const {
     const int i = 8 * c - off;
-    if (c < chunks && i >= 0 && i + 8 <= V) {
+    if (whole(c)) {
       if constexpr (sizeof(T) == 4) {
         const float4 a = *reinterpret_cast<const float4*>(x + i), b = *reinterpret_cast<const float4*>(x + i + 4);
         v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
@@ -144,13 +150,36 @@ struct Row {
           v[2 * k + 1] = f.y;
         }
       }
-      return;
-    }
+    } else {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      v[j] = -INFINITY;
-      if (c < chunks && i + j >= 0 && i + j < V) v[j] = to_float(x[i + j]);
+      for (int j = 0; j < 8; ++j) v[j] = -INFINITY;
+      if (c < chunks) {                  // at the ends of the row
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (i + j >= 0 && i + j < V) v[j] = to_float(x[i + j]);
+      }
     }
+    if (only_inf) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = v[j] == INFINITY ? 0.f : -INFINITY;
+    }
+  }
+  // the larger of m and the chunk's largest logit, NaN aside
+  __device__ __forceinline__ float max_with(int c, float m) const {
+    if constexpr (sizeof(T) == 2) {
+      if (whole(c)) {
+        const uint4 a = *reinterpret_cast<const uint4*>(x + 8 * c - off);
+        using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+        const T2* w = reinterpret_cast<const T2*>(&a);
+        const T2 y = __hmax2(__hmax2(w[0], w[1]), __hmax2(w[2], w[3]));
+        return fmaxf(m, fmaxf(to_float(y.x), to_float(y.y)));
+      }
+    }
+    float v[8];
+    load(c, v);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) m = fmaxf(m, v[j]);
+    return m;
   }
 };
 
@@ -160,14 +189,7 @@ __device__ __forceinline__ V warp_sum(V v) {
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
   return v;
 }
-__device__ __forceinline__ uint64_t warp_max(uint64_t v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const uint64_t c = __shfl_xor_sync(kFull, v, o);
-    v = c > v ? c : v;
-  }
-  return v;
-}
+__device__ __forceinline__ uint32_t warp_max(uint32_t v) { return __reduce_max_sync(kFull, v); }
 
 struct Cut {
   uint32_t key;         // images above are kept, those below are not
@@ -175,9 +197,10 @@ struct Cut {
 };
 
 struct Shared {
-  uint64_t warp_best[kWarps];
-  uint64_t best;                       // of this CTA: image << 32 | ~index
+  uint32_t warp_best[kWarps];
+  uint32_t best, first;                // of this CTA: largest image; ~(lowest index that has the row's largest)
   uint32_t bound;                      // of this CTA
+  uint64_t weight;                     // of this CTA, in fixed point
   double part[kWarps][kGranules];      // weight of each granule
   double part_sum[kWarps];
   double sum;                          // of this CTA
@@ -233,75 +256,86 @@ struct Sampler {
     return c < c1 ? c : row.chunks;
   }
 
-  // largest logit of the row (image << 32 | ~index); thread_key: this thread's largest image
-  __device__ __forceinline__ uint64_t largest(uint32_t& thread_key) {
-    float best = -INFINITY;
-    int at = 0;
+  // largest of a value over the row, through a field of Shared of its own
+  __device__ __forceinline__ uint32_t row_max(uint32_t v, uint32_t Shared::* field) {
+    v = warp_max(v);
+    __syncthreads();
+    if (lane == 0) sh.warp_best[warp] = v;
+    __syncthreads();
+    v = warp_max(sh.warp_best[lane & (kWarps - 1)]);
+    if (ctas == 1) return v;
+    if (threadIdx.x == 0) sh.*field = v;
+    cluster.sync();
+    return warp_max(of(lane & (ctas - 1)).*field);
+  }
+
+  // image of the largest logit of this thread
+  __device__ __forceinline__ uint32_t largest() {
+    float m = -INFINITY;
 #pragma unroll 4
-    for (int it = 0; it < iters; ++it) {
-      float v[8];
-      const int c = chunk(it);
-      row.load(c, v);
-      float m = -INFINITY;
+    for (int it = 0; it < iters; ++it) m = row.max_with(chunk(it), m);
+    return key_of(m);
+  }
+
+  // lowest index with the largest image
+  __device__ __forceinline__ uint32_t first_of(uint32_t kmax, uint32_t thread_key) {
+    uint32_t mine = 0;
+    if (thread_key == kmax) {
+#pragma unroll 1
+      for (int it = 0; it < iters && mine == 0; ++it) {
+        float v[8];
+        row.load(chunk(it), v);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) m = fmaxf(m, v[j]);      // drops NaN
-      if (m > best) {                                      // chunks come in index order
-        best = m;
-        at = c;
+        for (int j = 7; j >= 0; --j)
+          if (key_of(v[j]) == kmax) mine = ~static_cast<uint32_t>(row.index(chunk(it), j));
       }
     }
-    thread_key = key_of(best);
-    uint64_t mine = 0;
-    if (thread_key != 0) {
-      float v[8];
-      row.load(at, v);
-      int j = 7;
-#pragma unroll
-      for (int k = 7; k >= 0; --k)
-        if (v[k] == best) j = k;
-      mine = static_cast<uint64_t>(thread_key) << 32 | static_cast<uint32_t>(~static_cast<uint32_t>(row.index(at, j)));
-    }
-    mine = warp_max(mine);
-    if (lane == 0) sh.warp_best[warp] = mine;
-    __syncthreads();
-    uint64_t b = lane < kWarps ? sh.warp_best[lane] : 0;
-    b = warp_max(b);
-    if (ctas == 1) return b;
-    if (threadIdx.x == 0) sh.best = b;
-    cluster.sync();
-    b = lane < ctas ? of(lane).best : 0;
-    return warp_max(b);
+    __syncwarp();
+    return ~row_max(mine, &Shared::first);
   }
 
   // An image that at least k elements of the row reach: the k-th largest of a CTA's thread maxima (k <= kThreads), the
-  // largest of these over the CTAs. Bit by bit: the largest image that k threads reach.
+  // largest of these over the CTAs. Bit by bit the largest image that k threads reach, to 18 bits (all that a 16-bit
+  // type has but for two of fp16's; a bound that is too low by less than 2^-9 finds a few more candidates).
   __device__ __forceinline__ uint32_t bound_of_k(uint32_t thread_key, int k) {
     uint32_t b = 0;
-    for (int bit = 31; bit >= 0; --bit) {
+#pragma unroll 1
+    for (int bit = 31; bit >= 14; --bit) {
       const uint32_t t = b | (1u << bit);
       if (__syncthreads_count(thread_key >= t) >= k) b = t;
     }
     if (ctas == 1) return b;
     if (threadIdx.x == 0) sh.bound = b;
     cluster.sync();
-    b = lane < ctas ? of(lane).bound : 0;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) b = max(b, __shfl_xor_sync(kFull, b, o));
-    return b;
+    return warp_max(of(lane & (ctas - 1)).bound);
   }
 
-  // whether an element is kept: by the cut (ties: the first by index; tie_rank counts those of this warp's segment met so
-  // far, all lanes call) and by min_p
+  // what is kept: above the cut, and the first of its ties by index; weights of at least min_w
   struct Kept {
     Cut cut;
     double min_w;
   };
 
-  // weight of what is kept among the eight logits of each lane, in index order within the lane; w[j] = 0 for the others
+  // Weights of what is kept among the eight logits of each lane (w[j] = 0 for the others) and their sum, in index order.
+  // kAll: nothing is cut. tie_rank counts the ties of this warp's segment met so far. All lanes call.
+  template <bool kAll>
   __device__ __forceinline__ double weigh(const float (&v)[8], const Kept& kept, uint32_t& tie_rank, double (&w)[8]) {
     double s = 0.0;
-    uint32_t mine = 0, before = 0;
+    if constexpr (kAll) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const double x = weight.value(v[j]);
+        w[j] = 0.0;
+        if (weight.some(v[j])) {
+          w[j] = x;
+          s += x;
+        }
+      }
+      return s;
+    }
+    uint32_t before = 0;
     if (kept.cut.key != 0) {
+      uint32_t mine = 0;
 #pragma unroll
       for (int j = 0; j < 8; ++j) mine += key_of(v[j]) == kept.cut.key ? 1u : 0u;
       uint32_t inc = mine;
@@ -319,7 +353,7 @@ struct Sampler {
       const uint32_t k = key_of(v[j]);
       bool keep = k > kept.cut.key;
       if (kept.cut.key != 0 && k == kept.cut.key) keep = before++ < kept.cut.ties;
-      if (kept.cut.key != 0 && !__any_sync(kFull, keep)) continue;
+      if (!__any_sync(kFull, keep)) continue;
       const double x = weight(v[j]);
       if (keep && x >= kept.min_w) w[j] = x;
       s += w[j];
@@ -355,15 +389,23 @@ struct Sampler {
   }
 
   // weight of every granule; returns the row's
+  template <bool kAll>
   __device__ __forceinline__ double sums(const Kept& kept, uint32_t ties0) {
     uint32_t tie_rank = ties0;
+#pragma unroll 1
     for (int g = 0; g < kGranules; ++g) {
       double s = 0.0;
-      for (int it = g * step; it < min((g + 1) * step, iters); ++it) {
-        float v[8];
+      const int end = min((g + 1) * step, iters);
+      float v[8];
+      if (g * step < end) row.load(chunk(g * step), v);
+#pragma unroll 1
+      for (int it = g * step; it < end; ++it) {
+        float next[8];
         double w[8];
-        row.load(chunk(it), v);
-        s += weigh(v, kept, tie_rank, w);
+        row.load(it + 1 < end ? chunk(it + 1) : row.chunks, next);     // on its way meanwhile
+        s += weigh<kAll>(v, kept, tie_rank, w);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = next[j];
       }
       s = warp_sum(s);
       if (lane == 0) sh.part[warp][g] = s;
@@ -404,6 +446,7 @@ struct Sampler {
   }
 
   // draws by the granules' weights (sums() of the same `kept` came before)
+  template <bool kAll>
   __device__ __forceinline__ void draw(int64_t n, const Kept& kept, uint32_t ties0, double total) {
     const double r = fmin(fmax(static_cast<double>(p.u[n]), 0.0), 1.0 - 0x1p-24) * total;
     double before = 0.0;
@@ -413,7 +456,7 @@ struct Sampler {
     uint32_t tie_rank = ties0;
     float v[8];
     double w[8];
-    if (kept.cut.key != 0)                       // ties of the granules before
+    if (!kAll && kept.cut.key != 0)              // ties of the granules before
       for (int it = 0; it < g * step; ++it) {
         row.load(chunk(it), v);
         uint32_t t = 0;
@@ -425,7 +468,7 @@ struct Sampler {
     double found_w = 0.0;
     for (int it = g * step; it < min((g + 1) * step, iters); ++it) {
       row.load(chunk(it), v);
-      const double mine = weigh(v, kept, tie_rank, w);
+      const double mine = weigh<kAll>(v, kept, tie_rank, w);
       double inc = mine;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -470,17 +513,23 @@ struct Sampler {
   // the list is not written)
   __device__ __forceinline__ uint32_t gather(uint32_t bound, uint32_t thread_key) {
     const bool has = thread_key >= bound;
-    const bool any = __any_sync(kFull, has);
-    uint32_t n = 0;
-    if (any) {
+    uint32_t n = 0, where = 0;                   // iterations (mod 32) that have candidates
+    if (__any_sync(kFull, has)) {
 #pragma unroll 2
       for (int it = 0; it < iters; ++it) {
-        float v[8];
-        row.load(has ? chunk(it) : row.chunks, v);
+        uint32_t c = 0;
+        if (has) {
+          float v[8];
+          row.load(chunk(it), v);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) n += key_of(v[j]) >= bound ? 1u : 0u;
+          for (int j = 0; j < 8; ++j) c += key_of(v[j]) >= bound ? 1u : 0u;
+        }
+        n += c;
+        if (c != 0) where |= 1u << (it & 31);
       }
+      __syncwarp();
       n = warp_sum(n);
+      where = __reduce_or_sync(kFull, where);
     }
     if (lane == 0) sh.count[warp] = n;
     __syncthreads();
@@ -499,15 +548,16 @@ struct Sampler {
       }
     }
     if (all > kList) return all;
-    if (any && n > 0) {
+    if (n > 0) {
       Shared& to = ctas == 1 ? sh : *cluster.map_shared_rank(&sh, 0);
+#pragma unroll 1
       for (int it = 0; it < iters; ++it) {
+        if ((where >> (it & 31) & 1u) == 0) continue;
         float v[8];
         row.load(has ? chunk(it) : row.chunks, v);
         uint32_t mine = 0;
 #pragma unroll
         for (int j = 0; j < 8; ++j) mine += key_of(v[j]) >= bound ? 1u : 0u;
-        if (!__any_sync(kFull, mine != 0)) continue;
         uint32_t inc = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -531,9 +581,10 @@ struct Sampler {
     return all;
   }
 
-  // inclusive sum over the threads of the block before and with this one, in a fixed order
+  // inclusive sum over the threads of the block before and with this one, in a fixed order; only the first `used` warps
+  // have anything but zeros
   template <typename V>
-  __device__ __forceinline__ V block_scan(V v, V* scratch) {
+  __device__ __forceinline__ V block_scan(V v, V* scratch, int used = kWarps) {
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const V c = __shfl_up_sync(kFull, v, o);
@@ -543,59 +594,60 @@ struct Sampler {
     if (lane == 31) scratch[warp] = v;
     __syncthreads();
     V before = 0;
-    for (int i = 0; i < warp; ++i) before += scratch[i];
+#pragma unroll 1
+    for (int i = 0; i < min(warp, used); ++i) before += scratch[i];
     return before + v;
   }
 
   // Cuts and draws from the list of n candidates, which holds everything that can be kept. z: weight of what top_p is a
   // share of, or 0 where that is the first k candidates.
   __device__ __forceinline__ void draw_list(int64_t n_row, int n, int k, float top_p, double min_w, double z) {
-    const int t = threadIdx.x;
+    const int t = threadIdx.x, used = (n + 31) / 32;
     const bool have = t < n;
-    const uint32_t key = have ? sh.key[t] : 0u;
-    const double w = weight(have ? value_of(key) : -INFINITY);
-    // rank in descending order; the list is in index order, so ties are won by the earlier position
-    int rank_k = 0;
-#pragma unroll 8
-    for (int j = 0; j < n; ++j) {
-      const uint32_t o = sh.key[j];
-      rank_k += (o > key || (o == key && j < t)) ? 1 : 0;
-    }
-    if (have) {
-      sh.by_key[rank_k] = static_cast<uint32_t>(t);
-      sh.w[t] = w;
+    if (warp < used) {
+      const uint32_t key = have ? sh.key[t] : 0u;
+      const double w = weight(have ? value_of(key) : -INFINITY);
+      // rank in descending order; the list is in index order, so ties are won by the earlier position
+      int rank_k = 0;
+#pragma unroll 4
+      for (int j = 0; j < n; ++j) {
+        const uint32_t o = sh.key[j];
+        rank_k += (o > key || (o == key && j < t)) ? 1 : 0;
+      }
+      if (have) {
+        sh.by_key[rank_k] = static_cast<uint32_t>(t);
+        sh.w[t] = w;
+      }
     }
     __syncthreads();
-    double* scratch = sh.part_sum;
     // in the order of ranks: thread t looks at the candidate of rank t
     const int first = k > 0 ? min(k, n) : n;
     const int who = have ? static_cast<int>(sh.by_key[t]) : 0;
     const double wr = t < first ? sh.w[who] : 0.0;
-    const double inc = block_scan(wr, scratch);
-    __syncthreads();
-    if (t == kThreads - 1) sh.sum = inc;
-    __syncthreads();
-    const double share = static_cast<double>(top_p) * (z > 0.0 ? z : sh.sum);
-    bool keep = t < first && (t == 0 || top_p >= 1.f || inc - wr < share);
-    keep = keep && wr >= min_w;
+    bool keep = t < first && wr >= min_w;
+    if (top_p < 1.f) {
+      const double inc = block_scan(wr, sh.part_sum, used);
+      if (t == kThreads - 1) sh.sum = inc;
+      __syncthreads();
+      keep = keep && (t == 0 || inc - wr < static_cast<double>(top_p) * (z > 0.0 ? z : sh.sum));
+    }
     __syncthreads();
     if (have && !keep) sh.w[who] = 0.0;
     __syncthreads();
     // in index order
     const double wi = have ? sh.w[t] : 0.0;
-    const double run = block_scan(wi, scratch);
-    __syncthreads();
+    const double run = block_scan(wi, sh.part_sum, used);
     if (t == kThreads - 1) sh.sum = run;
     __syncthreads();
     const double total = sh.sum;
     const double r = fmin(fmax(static_cast<double>(p.u[n_row]), 0.0), 1.0 - 0x1p-24) * total;
     // first with run > r; rounding cannot hide the last one, whose running sum is `total` itself
-    const bool hit = wi > 0.0 && run > r;
-    const uint32_t m = __ballot_sync(kFull, hit);
+    const uint32_t m = __ballot_sync(kFull, wi > 0.0 && run > r);
     if (lane == 0) sh.count[warp] = m;
     __syncthreads();
     if (t == 0) {
-      for (int i = 0; i < kWarps; ++i) {
+#pragma unroll 1
+      for (int i = 0; i < used; ++i) {
         if (sh.count[i] == 0) continue;
         const int at = 32 * i + __ffs(sh.count[i]) - 1;
         write(n_row, static_cast<int>(sh.idx[at]), sh.w[at], total);
@@ -700,17 +752,22 @@ struct Sampler {
   }
 
   __device__ __forceinline__ void run(int64_t n) {
-    uint32_t thread_key;
-    const uint64_t best = largest(thread_key);
+    uint32_t thread_key = largest();
+    uint32_t kmax = row_max(thread_key, &Shared::best);
     const float t = p.temperature != nullptr ? p.temperature[n] : p.temperature_all;
-    const uint32_t kmax = static_cast<uint32_t>(best >> 32);
     const float mp = p.min_p != nullptr ? p.min_p[n] : p.min_p_all;
     if (kmax == 0 || !(t > 0.f) || !(mp <= 1.f)) {         // min_p above 1 leaves the largest alone
+      const uint32_t at = kmax != 0 ? first_of(kmax, thread_key) : 0u;
       if (rank == 0 && threadIdx.x == 0) {
-        p.token[n] = kmax == 0 ? -1 : static_cast<int64_t>(~static_cast<uint32_t>(best));
+        p.token[n] = kmax == 0 ? -1 : static_cast<int64_t>(at);
         if (p.logprob != nullptr) p.logprob[n] = kmax == 0 ? -INFINITY : 0.f;
       }
       return;
+    }
+    if (value_of(kmax) == INFINITY) {
+      row.only_inf = true;
+      thread_key = thread_key == kmax ? key_of(0.f) : 0u;
+      kmax = key_of(0.f);
     }
     weight.init(kmax, t);
     int64_t k64 = p.top_k_all;
@@ -725,11 +782,11 @@ struct Sampler {
     // images from `low` up hold everything that is kept; 1 is below all candidates
     uint32_t low = 1;
     double z = 0.0;
-    Kept all{Cut{0, 0}, 0.0};
+    const Kept all{Cut{0, 0}, 0.0};
     if (k > 0) {
       if (k <= kThreads) low = max(bound_of_k(thread_key, k), 1u);
     } else if (by_p) {
-      z = sums(all, 0);
+      z = sums<true>(all, 0);
       low = bound_of_weight((1.0 - share) * z / p.V);
     }
     if (min_w > 0.0 && !(k > 0 && by_p)) low = max(low, bound_of_weight(min_w));
@@ -762,10 +819,10 @@ struct Sampler {
       const double wt = weight(cut.key != 0 ? value_of(cut.key) : -INFINITY);
       sum = block_scan(sum, sh.scan);
       __syncthreads();
-      if (threadIdx.x == kThreads - 1) sh.best = sum;
+      if (threadIdx.x == kThreads - 1) sh.weight = sum;
       sync();
       sum = cut.ties * fixed(wt);
-      for (int r = 0; r < ctas; ++r) sum += of(r).best;
+      for (int r = 0; r < ctas; ++r) sum += of(r).weight;
       const double target = fmax(share * static_cast<double>(sum), 1.0);     // the largest is always kept
       const uint32_t key = radix_find<true>(cut, cut.key != 0 ? cut.key : 1, target, above, at);
       const uint64_t w = fixed(weight(value_of(key)));
@@ -780,9 +837,13 @@ struct Sampler {
       if (key == cut.key && cut.ties < ties) ties = cut.ties;
       cut = Cut{key, static_cast<uint32_t>(min(ties, static_cast<uint64_t>(0xffffffffu)))};
     }
+    if (cut.key == 0 && min_w == 0.0) {
+      draw<true>(n, all, 0, sums<true>(all, 0));
+      return;
+    }
     const Kept kept{cut, min_w};
     const uint32_t ties0 = ties_before(cut);
-    draw(n, kept, ties0, sums(kept, ties0));
+    draw<false>(n, kept, ties0, sums<false>(kept, ties0));
   }
 
   // an image that every weight >= w reaches (rounded down by more than its own and the weights' rounding)
