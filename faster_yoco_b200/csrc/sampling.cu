@@ -37,6 +37,7 @@ constexpr int kWarps = kThreads / 32;
 constexpr int kMaxCluster = 8;
 constexpr int kGranules = 8;        // pieces of a warp's segment whose weights are kept
 constexpr int kList = kThreads;     // candidates of the short list: one a thread
+constexpr int kGuess = 192;         // elements that a first look at a top-p cut is content with
 constexpr int kBinBits = 11;        // of a radix step
 constexpr uint32_t kFull = 0xffffffffu;
 
@@ -130,15 +131,31 @@ struct Row {
   }
   __device__ __forceinline__ int index(int c, int j) const { return 8 * c - off + j; }
   __device__ __forceinline__ bool whole(int c) const { return c < chunks && 8 * c >= off && 8 * c - off + 8 <= V; }
-  __device__ __forceinline__ void load(int c, float (&v)[8]) const {
+  // a chunk as it is stored, and its values: fetch() can run ahead
+  struct Raw {
+    uint4 a[sizeof(T) / 2];
+  };
+  __device__ __forceinline__ Raw fetch(int c) const {
+    Raw raw{};
+    if (whole(c)) {
+      const uint4* src = reinterpret_cast<const uint4*>(x + 8 * c - off);
+#pragma unroll
+      for (int k = 0; k < static_cast<int>(sizeof(T)) / 2; ++k) raw.a[k] = src[k];
+    }
+    return raw;
+  }
+  __device__ __forceinline__ void load(int c, float (&v)[8]) const { values(c, fetch(c), v); }
+  __device__ __forceinline__ void values(int c, const Raw& raw, float (&v)[8]) const {
     const int i = 8 * c - off;
     if (whole(c)) {
       if constexpr (sizeof(T) == 4) {
-        const float4 a = *reinterpret_cast<const float4*>(x + i), b = *reinterpret_cast<const float4*>(x + i + 4);
-        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          v[4 * k] = __uint_as_float(raw.a[k].x), v[4 * k + 1] = __uint_as_float(raw.a[k].y);
+          v[4 * k + 2] = __uint_as_float(raw.a[k].z), v[4 * k + 3] = __uint_as_float(raw.a[k].w);
+        }
       } else {
-        const uint4 a = *reinterpret_cast<const uint4*>(x + i);
-        const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+        const uint32_t w[4] = {raw.a[0].x, raw.a[0].y, raw.a[0].z, raw.a[0].w};
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           float2 f;
@@ -191,6 +208,9 @@ __device__ __forceinline__ V warp_sum(V v) {
 }
 __device__ __forceinline__ uint32_t warp_max(uint32_t v) { return __reduce_max_sync(kFull, v); }
 
+// What is kept of a row: everything, weights of at least min_p, or what a cut (and min_p) leaves
+enum Mode : int { kAll, kByWeight, kByCut };
+
 struct Cut {
   uint32_t key;         // images above are kept, those below are not
   uint32_t ties;        // how many images equal to `key` are kept (the first ones by index)
@@ -206,6 +226,7 @@ struct Shared {
   double sum;                          // of this CTA
   uint32_t count[kWarps];
   uint32_t total_count;                // of this CTA (candidates, or ties)
+  bool done;                           // a token was drawn from the list
   uint32_t hist_lo[1 << kBinBits], hist_hi[1 << kBinBits];
   uint64_t scan[kWarps];
   uint64_t found[3];
@@ -317,27 +338,27 @@ struct Sampler {
   };
 
   // Weights of what is kept among the eight logits of each lane (w[j] = 0 for the others) and their sum, in index order.
-  // kAll: nothing is cut. tie_rank counts the ties of this warp's segment met so far. All lanes call.
-  template <bool kAll>
+  // tie_rank counts the ties of this warp's segment met so far. All lanes call.
+  template <Mode kMode>
   __device__ __forceinline__ double weigh(const float (&v)[8], const Kept& kept, uint32_t& tie_rank, double (&w)[8]) {
     double s = 0.0;
-    if constexpr (kAll) {
+    if constexpr (kMode != kByCut) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const double x = weight.value(v[j]);
         w[j] = 0.0;
-        if (weight.some(v[j])) {
+        if (weight.some(v[j]) && (kMode == kAll || x >= kept.min_w)) {
           w[j] = x;
           s += x;
         }
       }
       return s;
     }
-    uint32_t before = 0;
-    if (kept.cut.key != 0) {
-      uint32_t mine = 0;
+    uint32_t mine = 0;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) mine += key_of(v[j]) == kept.cut.key ? 1u : 0u;
+    for (int j = 0; j < 8; ++j) mine += key_of(v[j]) == kept.cut.key ? 1u : 0u;
+    uint32_t before = 0;
+    if (__any_sync(kFull, mine != 0)) {
       uint32_t inc = mine;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -352,7 +373,7 @@ struct Sampler {
       w[j] = 0.0;
       const uint32_t k = key_of(v[j]);
       bool keep = k > kept.cut.key;
-      if (kept.cut.key != 0 && k == kept.cut.key) keep = before++ < kept.cut.ties;
+      if (k == kept.cut.key) keep = before++ < kept.cut.ties;
       if (!__any_sync(kFull, keep)) continue;
       const double x = weight(v[j]);
       if (keep && x >= kept.min_w) w[j] = x;
@@ -363,7 +384,6 @@ struct Sampler {
 
   // ties of the cut before this warp's segment
   __device__ __forceinline__ uint32_t ties_before(const Cut& cut) {
-    if (cut.key == 0) return 0;
     uint32_t n = 0;
 #pragma unroll 2
     for (int it = 0; it < iters; ++it) {
@@ -389,23 +409,22 @@ struct Sampler {
   }
 
   // weight of every granule; returns the row's
-  template <bool kAll>
+  template <Mode kMode>
   __device__ __forceinline__ double sums(const Kept& kept, uint32_t ties0) {
     uint32_t tie_rank = ties0;
 #pragma unroll 1
     for (int g = 0; g < kGranules; ++g) {
       double s = 0.0;
       const int end = min((g + 1) * step, iters);
-      float v[8];
-      if (g * step < end) row.load(chunk(g * step), v);
+      typename Row<T>::Raw raw[2] = {row.fetch(chunk(g * step)), row.fetch(chunk(g * step + 1))};
 #pragma unroll 1
       for (int it = g * step; it < end; ++it) {
-        float next[8];
+        float v[8];
         double w[8];
-        row.load(it + 1 < end ? chunk(it + 1) : row.chunks, next);     // on its way meanwhile
-        s += weigh<kAll>(v, kept, tie_rank, w);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = next[j];
+        row.values(chunk(it), raw[0], v);
+        raw[0] = raw[1];
+        raw[1] = row.fetch(chunk(it + 2));       // two chunks are on their way meanwhile
+        s += weigh<kMode>(v, kept, tie_rank, w);
       }
       s = warp_sum(s);
       if (lane == 0) sh.part[warp][g] = s;
@@ -446,7 +465,7 @@ struct Sampler {
   }
 
   // draws by the granules' weights (sums() of the same `kept` came before)
-  template <bool kAll>
+  template <Mode kMode>
   __device__ __forceinline__ void draw(int64_t n, const Kept& kept, uint32_t ties0, double total) {
     const double r = fmin(fmax(static_cast<double>(p.u[n]), 0.0), 1.0 - 0x1p-24) * total;
     double before = 0.0;
@@ -456,7 +475,7 @@ struct Sampler {
     uint32_t tie_rank = ties0;
     float v[8];
     double w[8];
-    if (!kAll && kept.cut.key != 0)              // ties of the granules before
+    if (kMode == kByCut)                         // ties of the granules before
       for (int it = 0; it < g * step; ++it) {
         row.load(chunk(it), v);
         uint32_t t = 0;
@@ -468,7 +487,7 @@ struct Sampler {
     double found_w = 0.0;
     for (int it = g * step; it < min((g + 1) * step, iters); ++it) {
       row.load(chunk(it), v);
-      const double mine = weigh<kAll>(v, kept, tie_rank, w);
+      const double mine = weigh<kMode>(v, kept, tie_rank, w);
       double inc = mine;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -599,9 +618,10 @@ struct Sampler {
     return before + v;
   }
 
-  // Cuts and draws from the list of n candidates, which holds everything that can be kept. z: weight of what top_p is a
-  // share of, or 0 where that is the first k candidates.
-  __device__ __forceinline__ void draw_list(int64_t n_row, int n, int k, float top_p, double min_w, double z) {
+  // Cuts and draws from the list of n candidates, which holds everything that can be kept (sure), or all larger images of
+  // what it holds: then false if their weight does not reach the share. z: weight of what top_p is a share of, or 0 where
+  // that is the first k candidates.
+  __device__ __forceinline__ bool draw_list(int64_t n_row, int n, int k, float top_p, double min_w, double z, bool sure) {
     const int t = threadIdx.x, used = (n + 31) / 32;
     const bool have = t < n;
     if (warp < used) {
@@ -629,6 +649,7 @@ struct Sampler {
       const double inc = block_scan(wr, sh.part_sum, used);
       if (t == kThreads - 1) sh.sum = inc;
       __syncthreads();
+      if (!sure && sh.sum < static_cast<double>(top_p) * z) return false;
       keep = keep && (t == 0 || inc - wr < static_cast<double>(top_p) * (z > 0.0 ? z : sh.sum));
     }
     __syncthreads();
@@ -654,6 +675,7 @@ struct Sampler {
         break;
       }
     }
+    return true;
   }
 
   __device__ __forceinline__ uint64_t fixed(double w) const { return static_cast<uint64_t>(__double2ll_rn(w * p.unit)); }
@@ -780,21 +802,34 @@ struct Sampler {
     const double min_w = mp > 0.f ? static_cast<double>(mp) : 0.0;
 
     // images from `low` up hold everything that is kept; 1 is below all candidates
-    uint32_t low = 1;
+    uint32_t low = 1, guess = 1;
     double z = 0.0;
     const Kept all{Cut{0, 0}, 0.0};
     if (k > 0) {
       if (k <= kThreads) low = max(bound_of_k(thread_key, k), 1u);
     } else if (by_p) {
-      z = sums<true>(all, 0);
+      z = sums<kAll>(all, 0);
       low = bound_of_weight((1.0 - share) * z / p.V);
+      // that bound is far too low for a steep distribution: try what about kGuess elements reach, and see whether they
+      // weigh enough
+      guess = bound_of_k(thread_key, kGuess / ctas);
     }
     if (min_w > 0.0 && !(k > 0 && by_p)) low = max(low, bound_of_weight(min_w));
-    if (low > 1 || p.V <= kList) {
-      const uint32_t c = gather(low, thread_key);
+    if (low > 1 || guess > 1 || p.V <= kList) {
+      const bool sure = guess <= low;
+      const uint32_t c = gather(max(low, guess), thread_key);
       if (c <= kList) {
-        if (rank == 0) draw_list(n, static_cast<int>(c), k, by_p ? static_cast<float>(share) : 1.f, min_w, z);
-        return;
+        if (sure) {
+          if (rank == 0)
+            draw_list(n, static_cast<int>(c), k, by_p ? static_cast<float>(share) : 1.f, min_w, z, true);
+          return;
+        }
+        if (rank == 0) {
+          const bool done = draw_list(n, static_cast<int>(c), 0, static_cast<float>(share), min_w, z, false);
+          if (threadIdx.x == 0) sh.done = done;
+        }
+        sync();
+        if (of(0).done) return;
       }
     }
     Cut cut{0, 0};
@@ -805,26 +840,30 @@ struct Sampler {
       cut = Cut{key, static_cast<uint32_t>(min(left, at))};
     }
     if (by_p) {
-      // shares of fixed-point sums, so that the search and its target agree
-      uint64_t sum = 0;
-      for (int it = 0; it < iters; ++it) {
-        float v[8];
-        row.load(chunk(it), v);
+      double kept_weight = z * p.unit;             // in fixed-point units
+      if (k > 0) {
+        uint64_t sum = 0;
+        for (int it = 0; it < iters; ++it) {
+          float v[8];
+          row.load(chunk(it), v);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const uint64_t a = fixed(weight(v[j]));
-          sum += key_of(v[j]) > cut.key ? a : 0;
+          for (int j = 0; j < 8; ++j) {
+            const uint64_t a = fixed(weight(v[j]));
+            sum += key_of(v[j]) > cut.key ? a : 0;
+          }
         }
+        const double wt = weight(value_of(cut.key));
+        sum = block_scan(sum, sh.scan);
+        __syncthreads();
+        if (threadIdx.x == kThreads - 1) sh.weight = sum;
+        sync();
+        sum = cut.ties * fixed(wt);
+        for (int r = 0; r < ctas; ++r) sum += of(r).weight;
+        kept_weight = static_cast<double>(sum);
+        low = cut.key;
       }
-      const double wt = weight(cut.key != 0 ? value_of(cut.key) : -INFINITY);
-      sum = block_scan(sum, sh.scan);
-      __syncthreads();
-      if (threadIdx.x == kThreads - 1) sh.weight = sum;
-      sync();
-      sum = cut.ties * fixed(wt);
-      for (int r = 0; r < ctas; ++r) sum += of(r).weight;
-      const double target = fmax(share * static_cast<double>(sum), 1.0);     // the largest is always kept
-      const uint32_t key = radix_find<true>(cut, cut.key != 0 ? cut.key : 1, target, above, at);
+      const double target = fmax(share * kept_weight, 1.0);      // the largest is always kept
+      const uint32_t key = radix_find<true>(cut, low, target, above, at);
       const uint64_t w = fixed(weight(value_of(key)));
       uint64_t ties = 1;
       if (w > 0 && target > static_cast<double>(above)) {
@@ -837,13 +876,15 @@ struct Sampler {
       if (key == cut.key && cut.ties < ties) ties = cut.ties;
       cut = Cut{key, static_cast<uint32_t>(min(ties, static_cast<uint64_t>(0xffffffffu)))};
     }
-    if (cut.key == 0 && min_w == 0.0) {
-      draw<true>(n, all, 0, sums<true>(all, 0));
-      return;
-    }
     const Kept kept{cut, min_w};
-    const uint32_t ties0 = ties_before(cut);
-    draw<false>(n, kept, ties0, sums<false>(kept, ties0));
+    if (cut.key != 0) {
+      const uint32_t ties0 = ties_before(cut);
+      draw<kByCut>(n, kept, ties0, sums<kByCut>(kept, ties0));
+    } else if (min_w > 0.0) {
+      draw<kByWeight>(n, kept, 0, sums<kByWeight>(kept, 0));
+    } else {
+      draw<kAll>(n, kept, 0, sums<kAll>(kept, 0));
+    }
   }
 
   // an image that every weight >= w reaches (rounded down by more than its own and the weights' rounding)
