@@ -156,6 +156,7 @@ at::Tensor status_tensor() {
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "faster_yoco_b200 sm_100a kernels";
+  pybind11::register_exception<fyb::Unsuitable>(m, "Unsuitable", PyExc_RuntimeError);
   m.def("gemm", &fyb::gemm, "C = A @ B^T on tcgen05 (operands K-major or MN-major)", py::arg("A"), py::arg("B"),
         py::arg("C"), py::arg("a_mn_major"), py::arg("b_mn_major"), py::arg("residual") = py::none());
   m.def("gemm_pair", &fyb::gemm_pair, "C = A @ B^T on CTA pairs (tcgen05.mma.cta_group::2, 256 x bn tiles)",

@@ -21,6 +21,15 @@ namespace fyb {
     if (!(cond)) throw std::runtime_error(std::string("faster_yoco_b200: ") + (msg)); \
   } while (0)
 
+// Arguments that a kernel cannot take as they are (a type, a shape, a layout): Python sees `Unsuitable`, a RuntimeError
+struct Unsuitable : std::runtime_error {
+  using std::runtime_error::runtime_error;
+};
+#define FYB_SUITS(cond, msg)                                                   \
+  do {                                                                         \
+    if (!(cond)) throw Unsuitable(std::string("faster_yoco_b200: ") + (msg)); \
+  } while (0)
+
 #define FYB_CUDA(call)                                                                               \
   do {                                                                                               \
     cudaError_t e_ = (call);                                                                         \

@@ -906,8 +906,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
 const void* row_param(const c10::optional<at::Tensor>& t, const at::Tensor& logits, at::ScalarType type,
                       const char* name) {
   if (!t.has_value() || !t->defined()) return nullptr;
-  FYB_CHECK(t->device() == logits.device() && t->scalar_type() == type && t->is_contiguous() &&
-                t->numel() == logits.size(0),
+  FYB_SUITS(t->device() == logits.device() && t->scalar_type() == type && t->dim() == 1 &&
+                t->is_contiguous() && t->size(0) == logits.size(0),
             std::string("sample: ") + name);
   return t->data_ptr();
 }
@@ -936,11 +936,11 @@ std::vector<at::Tensor> sample(const at::Tensor& logits, const at::Tensor& u,
                                const c10::optional<at::Tensor>& top_p, double top_p_all,
                                const c10::optional<at::Tensor>& min_p, double min_p_all, bool want_logprob) {
   FYB_RANGE("fyb::sample");
-  FYB_CHECK(logits.is_cuda() && logits.dim() == 2 && (logits.stride(1) == 1 || logits.size(1) == 1),
+  FYB_SUITS(logits.is_cuda() && logits.dim() == 2 && (logits.stride(1) == 1 || logits.size(1) == 1),
             "sample: logits [N, V] with a contiguous last dim expected");
   const int64_t N = logits.size(0), V = logits.size(1);
-  FYB_CHECK(V >= 1 && V < (1ll << 30) && N < (1ll << 27), "sample: sizes");
-  FYB_CHECK(logits.scalar_type() == at::kBFloat16 || logits.scalar_type() == at::kHalf ||
+  FYB_SUITS(V >= 1 && V < (1ll << 30) && N < (1ll << 27), "sample: sizes");
+  FYB_SUITS(logits.scalar_type() == at::kBFloat16 || logits.scalar_type() == at::kHalf ||
                 logits.scalar_type() == at::kFloat,
             "sample: bf16, fp16 or fp32 logits expected");
   c10::cuda::CUDAGuard guard(logits.device());
@@ -948,7 +948,8 @@ std::vector<at::Tensor> sample(const at::Tensor& logits, const at::Tensor& u,
   p.logits = logits.data_ptr();
   p.ld = logits.stride(0);
   p.V = static_cast<int>(V);
-  FYB_CHECK(u.device() == logits.device() && u.scalar_type() == at::kFloat && u.is_contiguous() && u.numel() == N,
+  FYB_SUITS(u.device() == logits.device() && u.scalar_type() == at::kFloat && u.dim() == 1 && u.is_contiguous() &&
+                u.size(0) == N,
             "sample: u");
   p.u = u.data_ptr<float>();
   p.temperature = static_cast<const float*>(row_param(temperature, logits, at::kFloat, "temperature"));

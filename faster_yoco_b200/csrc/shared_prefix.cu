@@ -27,6 +27,8 @@
 #include <c10/util/Optional.h>
 #include <cuda_fp16.h>
 
+#include <atomic>
+
 #include "common/host.h"
 #include "common/ptx.cuh"
 
@@ -702,13 +704,13 @@ __global__ void __launch_bounds__(kJoinCols * Parts * 32) spa_join_kernel(const 
 }
 
 View view_of(const at::Tensor& t, const at::Tensor& q, const char* name) {
-  FYB_CHECK(t.device() == q.device() && t.scalar_type() == q.scalar_type() && t.dim() == 4 &&
+  FYB_SUITS(t.device() == q.device() && t.scalar_type() == q.scalar_type() && t.dim() == 4 &&
                 t.size(3) == q.size(3) && t.stride(3) == 1,
             std::string("shared_prefix_attention: ") + name);
-  FYB_CHECK(reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0,
+  FYB_SUITS(reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0,
             std::string("shared_prefix_attention: 16-byte aligned ") + name);
   for (int d = 0; d < 3; ++d)
-    FYB_CHECK(t.size(d) <= 1 || (t.stride(d) > 0 && t.stride(d) % 8 == 0),
+    FYB_SUITS(t.size(d) <= 1 || (t.stride(d) > 0 && t.stride(d) % 8 == 0),
               std::string("shared_prefix_attention: strides of ") + name + " must be positive multiples of 8 elements");
   return View{t.data_ptr(), t.stride(0), t.stride(1), t.stride(2)};
 }
@@ -735,7 +737,7 @@ const void* length_ptr(const c10::optional<at::Tensor>& t, const at::Tensor& q, 
   wide = 0;
   if (!t.has_value() || !t->defined()) return nullptr;
   wide = t->scalar_type() == at::kLong;
-  FYB_CHECK(t->device() == q.device() && (wide || t->scalar_type() == at::kInt) && t->dim() == 1 && t->size(0) == n &&
+  FYB_SUITS(t->device() == q.device() && (wide || t->scalar_type() == at::kInt) && t->dim() == 1 && t->size(0) == n &&
                 (n <= 1 || t->stride(0) == 1),
             "shared_prefix_attention: lengths");
   return t->data_ptr();
@@ -744,8 +746,14 @@ const void* length_ptr(const c10::optional<at::Tensor>& t, const at::Tensor& q, 
 template <typename T, int D>
 void launch(const CUtensorMap& pk, const CUtensorMap& pv, const CUtensorMap& k, const CUtensorMap& v,
             const PrefixParams& p) {
-  // per call: the attribute belongs to the device that is current
-  FYB_CUDA(cudaFuncSetAttribute(spa_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, spa_smem<D>()));
+  // once for each device: the attribute belongs to the one that is current
+  static std::atomic<uint64_t> done{0};
+  int dev;
+  FYB_CUDA(cudaGetDevice(&dev));
+  if (dev >= 64 || (done.load(std::memory_order_acquire) >> dev & 1u) == 0) {
+    FYB_CUDA(cudaFuncSetAttribute(spa_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, spa_smem<D>()));
+    if (dev < 64) done.fetch_or(1ull << dev, std::memory_order_release);
+  }
   spa_kernel<T, D><<<p.ctas, kSpaThreads, spa_smem<D>(), cur_stream()>>>(pk, pv, k, v, p);
   check_launch("shared_prefix_attention");
   const int groups = p.G * p.Hk * ((p.rows_p + 7) / 8);
@@ -766,10 +774,10 @@ at::Tensor shared_prefix_attention(const at::Tensor& q, const at::Tensor& pk, co
                                    const c10::optional<at::Tensor>& lengths,
                                    const c10::optional<at::Tensor>& prefix_lengths, double scale) {
   FYB_RANGE("fyb::shared_prefix_attention");
-  FYB_CHECK(q.is_cuda() && q.dim() == 4 && (q.size(3) == 64 || q.size(3) == 128) &&
+  FYB_SUITS(q.is_cuda() && q.dim() == 4 && (q.size(3) == 64 || q.size(3) == 128) &&
                 (q.scalar_type() == at::kBFloat16 || q.scalar_type() == at::kHalf),
             "shared_prefix_attention: bf16 or fp16 q [B, Lq, Hq, 64 or 128] expected");
-  FYB_CHECK(scale > 0 && std::isfinite(scale), "shared_prefix_attention: scale must be positive");
+  FYB_SUITS(scale > 0 && std::isfinite(scale), "shared_prefix_attention: scale must be positive");
   const int64_t B = q.size(0), Lq = q.size(1), Hq = q.size(2), D = q.size(3);
   PrefixParams p{};
   p.q = view_of(q, q, "q");
@@ -778,10 +786,10 @@ at::Tensor shared_prefix_attention(const at::Tensor& q, const at::Tensor& pk, co
   view_of(k, q, "k");
   view_of(v, q, "v");
   const int64_t G = pk.size(0), P = pk.size(1), Hk = pk.size(2), S = k.size(1);
-  FYB_CHECK(pv.sizes() == pk.sizes() && v.sizes() == k.sizes() && k.size(0) == B && k.size(2) == Hk && Hk > 0 && G > 0 &&
+  FYB_SUITS(pv.sizes() == pk.sizes() && v.sizes() == k.sizes() && k.size(0) == B && k.size(2) == Hk && Hk > 0 && G > 0 &&
                 Hq > 0 && Hq % Hk == 0 && B % G == 0,
             "shared_prefix_attention: shape mismatch");
-  FYB_CHECK(B * Lq * Hq < (1ll << 31) && P < (1ll << 30) && S < (1ll << 30), "shared_prefix_attention: sizes");
+  FYB_SUITS(B * Lq * Hq < (1ll << 31) && P < (1ll << 30) && S < (1ll << 30), "shared_prefix_attention: sizes");
   c10::cuda::CUDAGuard guard(q.device());
   auto o = at::empty({B, Lq, Hq, D}, q.options());
   if (o.numel() == 0) return o;
@@ -799,7 +807,7 @@ at::Tensor shared_prefix_attention(const at::Tensor& q, const at::Tensor& pk, co
   int total[3];
   for (int c = 0; c < 3; ++c) {
     const int64_t tiles = segs[c] * (c == 2 ? p.tiles_o : p.tiles_p);
-    FYB_CHECK(tiles < (1ll << 31), "shared_prefix_attention: more than 2^31 tiles");
+    FYB_SUITS(tiles < (1ll << 31), "shared_prefix_attention: more than 2^31 tiles");
     total[c] = (int)tiles;
   }
   p.ctas = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;

@@ -556,6 +556,16 @@ def shared_prefix_attention(q: torch.Tensor, prefix_k: torch.Tensor, prefix_v: t
     The sm_100a kernel takes bf16 and fp16 with D 64 or 128; other types and sizes run the PyTorch expression. Key / value tensors are read in place when their rows are 16-byte
     aligned, else copied first. A value that SOME query of a row sees has to be finite. Inference only."""
     _no_grad_op("shared_prefix_attention", q, prefix_k, prefix_v, k, v)
+    scale = max(q.shape[-1], 1) ** -0.5 if scale is None else float(scale)
+    if not 0.0 < scale < math.inf:
+        raise ValueError(f"shared_prefix_attention: scale = {scale} must be positive and finite")
+    native = native_on(q)
+    if native:
+        try:
+            # the kernel checks what it is given
+            return _C().shared_prefix_attention(q, prefix_k, prefix_v, k, v, lengths, prefix_lengths, scale)
+        except _C().Unsuitable:
+            pass                                     # told below, or made suitable
     kv = (prefix_k, prefix_v, k, v)
     if any(t.dim() != 4 for t in (q, *kv)):
         raise ValueError("shared_prefix_attention: q, prefix_k, prefix_v, k and v have four dimensions")
@@ -572,10 +582,7 @@ def shared_prefix_attention(q: torch.Tensor, prefix_k: torch.Tensor, prefix_v: t
     for t, m, what in ((lengths, B, "lengths"), (prefix_lengths, G, "prefix_lengths")):
         if t is not None and (t.shape != (m,) or t.dtype not in (torch.int32, torch.int64) or t.device != q.device):
             raise ValueError(f"shared_prefix_attention: {what} must be int32 or int64 [{m}] on {q.device}")
-    scale = D ** -0.5 if scale is None else float(scale)
-    if not 0.0 < scale < math.inf:
-        raise ValueError(f"shared_prefix_attention: scale = {scale} must be positive and finite")
-    if native_on(q) and q.dtype in (torch.bfloat16, torch.float16) and D in (64, 128):
+    if native and q.dtype in (torch.bfloat16, torch.float16) and D in (64, 128):
         lengths, prefix_lengths = (t if t is None else t.contiguous() for t in (lengths, prefix_lengths))
         return _C().shared_prefix_attention(_vec16(q), *(_vec16(t) for t in kv), lengths, prefix_lengths, scale)
     return ref.shared_prefix_attention(q, *kv, lengths, prefix_lengths, scale)
@@ -602,6 +609,24 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0, top_
     ``return_logprob`` also the fp32 log-probability of each token under the distribution it was drawn from. Weights
     and their sums are held in 64 bits, so tokens do not depend on how the work is divided."""
     _no_grad_op("sample", logits)
+    native = native_on(logits)
+    numbers = []
+    for name, x, lo, hi in (("temperature", temperature, 0.0, math.inf), ("top_k", top_k, -2 ** 62, 2 ** 62),
+                            ("top_p", top_p, 0.0, math.inf), ("min_p", min_p, 0.0, 1.0)):
+        if isinstance(x, torch.Tensor):
+            numbers.append((x, 0))
+        elif lo <= x <= hi:
+            numbers.append((None, min(max(int(x), 0), 1 << 40) if name == "top_k" else float(x)))
+        else:
+            raise ValueError(f"sample: {name} = {x} is outside [{lo}, {hi}]")
+    (t, t1), (k, k1), (p, p1), (m, m1) = numbers
+    if native:
+        try:
+            # the kernel checks what it is given
+            tok, lp = _C().sample(logits, u, t, t1, k, k1, p, p1, m, m1, return_logprob)
+            return (tok, lp) if return_logprob else tok
+        except _C().Unsuitable:
+            pass                                     # told below, or made suitable
     if logits.dim() < 1 or logits.shape[-1] < 1:
         raise ValueError(f"sample: logits {tuple(logits.shape)} must be [..., V] with at least one token")
     if logits.dtype not in (torch.bfloat16, torch.float16, torch.float32):
@@ -610,22 +635,18 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0, top_
     if u.shape != lead or u.dtype != torch.float32 or u.device != logits.device:
         raise ValueError(f"sample: u must be fp32 {tuple(lead)} on {logits.device}")
     pars = []
-    for name, x, lo, hi in (("temperature", temperature, 0.0, math.inf), ("top_k", top_k, -math.inf, math.inf),
-                            ("top_p", top_p, 0.0, math.inf), ("min_p", min_p, 0.0, 1.0)):
-        if isinstance(x, torch.Tensor):
+    for name, (x, number) in zip(("temperature", "top_k", "top_p", "min_p"), numbers):
+        if x is not None:
             types = (torch.int32, torch.int64) if name == "top_k" else (torch.float32,)
             if x.shape != lead or x.dtype not in types or x.device != logits.device:
                 raise ValueError(f"sample: {name} must be a number or {types[0]} {tuple(lead)} on {logits.device}")
-            pars.append((x.reshape(-1).contiguous(), 0))
-            continue
-        if not lo <= x <= hi:
-            raise ValueError(f"sample: {name} = {x} is outside [{lo}, {hi}]")
-        pars.append((None, min(max(int(x), 0), V) if name == "top_k" else float(x)))
+            x = x.reshape(-1).contiguous()
+        pars.append((x, number))
     rows = logits if logits.dim() == 2 else logits.reshape(-1, V)
     uu = u.reshape(-1).contiguous()
-    if native_on(logits):
+    if native:
         rows = rows if rows.stride(1) == 1 or V == 1 else rows.contiguous()
-        tok, lp = _C().sample(rows, uu, *(y for x in pars for y in x), bool(return_logprob))
+        tok, lp = _C().sample(rows, uu, *(y for x in pars for y in x), return_logprob)
     else:
         full = [t if t is not None else torch.full((rows.shape[0],), x, device=rows.device,
                                                    dtype=torch.int64 if i == 1 else torch.float32)
