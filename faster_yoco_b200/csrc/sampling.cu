@@ -233,7 +233,9 @@ struct Shared {
   // the short list, in the CTA that draws from it
   uint32_t key[kList], idx[kList];
   double w[kList];
-  uint32_t by_key[kList];              // list position by rank
+  uint32_t listed;                     // candidates met
+  uint32_t by_key[kList];              // rank by index, by rank in descending order
+  uint32_t by_idx[kList];              // index, by rank by index (as the weights)
 };
 
 // What the CTAs of a row know of one another goes through a field of Shared that each writes once before a cluster barrier
@@ -293,8 +295,8 @@ struct Sampler {
   // image of the largest logit of this thread
   __device__ __forceinline__ uint32_t largest() {
     float m = -INFINITY;
-#pragma unroll 4
-    for (int it = 0; it < iters; ++it) m = row.max_with(chunk(it), m);
+#pragma unroll 8
+    for (int it = 0; it < iters; ++it) m = row.max_with(chunk(it), m);      // 64 KB of a CTA's slice in flight
     return key_of(m);
   }
 
@@ -315,9 +317,9 @@ struct Sampler {
     return ~row_max(mine, &Shared::first);
   }
 
-  // An image that at least k elements of the row reach: the k-th largest of a CTA's thread maxima (k <= kThreads), the
-  // largest of these over the CTAs. Bit by bit the largest image that k threads reach, to 18 bits (all that a 16-bit
-  // type has but for two of fp16's; a bound that is too low by less than 2^-9 finds a few more candidates).
+  // An image that at least k elements of the CTA's slice reach: the k-th largest of its thread maxima (k <= kThreads), bit
+  // by bit the largest image that k threads reach, to 18 bits (all that a 16-bit type has but for one of fp16's; a
+  // bound that is too low by less than 2^-9 finds a few more candidates).
   __device__ __forceinline__ uint32_t bound_of_k(uint32_t thread_key, int k) {
     uint32_t b = 0;
 #pragma unroll 1
@@ -325,6 +327,10 @@ struct Sampler {
       const uint32_t t = b | (1u << bit);
       if (__syncthreads_count(thread_key >= t) >= k) b = t;
     }
+    return max(b, 1u);
+  }
+  // the largest of the CTAs' bounds
+  __device__ __forceinline__ uint32_t shared_bound(uint32_t b) {
     if (ctas == 1) return b;
     if (threadIdx.x == 0) sh.bound = b;
     cluster.sync();
@@ -412,8 +418,9 @@ struct Sampler {
   template <Mode kMode>
   __device__ __forceinline__ double sums(const Kept& kept, uint32_t ties0) {
     uint32_t tie_rank = ties0;
+    double mine = 0.0;
 #pragma unroll 1
-    for (int g = 0; g < kGranules; ++g) {
+    for (int g = 0; g < kGranules && g * step < iters; ++g) {
       double s = 0.0;
       const int end = min((g + 1) * step, iters);
       typename Row<T>::Raw raw[2] = {row.fetch(chunk(g * step)), row.fetch(chunk(g * step + 1))};
@@ -428,22 +435,15 @@ struct Sampler {
       }
       s = warp_sum(s);
       if (lane == 0) sh.part[warp][g] = s;
+      mine += s;
     }
+    if (lane == 0) sh.part_sum[warp] = mine;
     __syncthreads();
-    if (lane == 0) {
-      double s = 0.0;
-      for (int g = 0; g < kGranules; ++g) s += sh.part[warp][g];
-      sh.part_sum[warp] = s;
-    }
-    __syncthreads();
-    double s = 0.0;
-    for (int i = 0; i < kWarps; ++i) s += sh.part_sum[i];
+    double s = warp_sum(lane < kWarps ? sh.part_sum[lane] : 0.0);
     if (ctas == 1) return s;
     if (threadIdx.x == 0) sh.sum = s;
     cluster.sync();
-    s = 0.0;
-    for (int r = 0; r < ctas; ++r) s += of(r).sum;
-    return s;
+    return warp_sum(lane < ctas ? of(lane).sum : 0.0);
   }
 
   // first of n parts whose running sum (from `before`) passes r, the last with any weight if rounding hides it
@@ -471,7 +471,7 @@ struct Sampler {
     double before = 0.0;
     if (ctas > 1 && pass(ctas, [&](int i) { return of(i).sum; }, r, before) != rank) return;
     if (pass(kWarps, [&](int i) { return sh.part_sum[i]; }, r, before) != warp) return;
-    const int g = pass(kGranules, [&](int i) { return sh.part[warp][i]; }, r, before);
+    const int g = pass((iters + step - 1) / step, [&](int i) { return sh.part[warp][i]; }, r, before);
     uint32_t tie_rank = ties0;
     float v[8];
     double w[8];
@@ -528,52 +528,25 @@ struct Sampler {
     if (p.logprob != nullptr) p.logprob[n] = static_cast<float>(log(w / total));
   }
 
-  // Candidates of image >= bound, in index order in the first CTA's list; returns how many there are (more than kList:
-  // the list is not written)
+  // Candidates of image >= bound (a CTA's own) to the first CTA's list, in no order; returns how many there are (more than
+  // kList: the list is short of some)
   __device__ __forceinline__ uint32_t gather(uint32_t bound, uint32_t thread_key) {
+    Shared& to = ctas == 1 ? sh : *cluster.map_shared_rank(&sh, 0);
     const bool has = thread_key >= bound;
-    uint32_t n = 0, where = 0;                   // iterations (mod 32) that have candidates
     if (__any_sync(kFull, has)) {
-#pragma unroll 2
-      for (int it = 0; it < iters; ++it) {
-        uint32_t c = 0;
-        if (has) {
-          float v[8];
-          row.load(chunk(it), v);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) c += key_of(v[j]) >= bound ? 1u : 0u;
-        }
-        n += c;
-        if (c != 0) where |= 1u << (it & 31);
+      uint32_t where = 0;                        // iterations (mod 32) that have candidates
+      if (has && *static_cast<volatile uint32_t*>(&to.listed) <= kList) {
+#pragma unroll 8
+        for (int it = 0; it < iters; ++it)
+          if (key_of(row.max_with(chunk(it), -INFINITY)) >= bound) where |= 1u << (it & 31);
       }
       __syncwarp();
-      n = warp_sum(n);
-      where = __reduce_or_sync(kFull, where);
-    }
-    if (lane == 0) sh.count[warp] = n;
-    __syncthreads();
-    uint32_t before = 0, all = 0;
-    for (int i = 0; i < kWarps; ++i) {
-      if (i < warp) before += sh.count[i];
-      all += sh.count[i];
-    }
-    if (ctas > 1) {
-      if (threadIdx.x == 0) sh.total_count = all;
-      cluster.sync();
-      all = 0;
-      for (int r = 0; r < ctas; ++r) {
-        if (r < rank) before += of(r).total_count;
-        all += of(r).total_count;
-      }
-    }
-    if (all > kList) return all;
-    if (n > 0) {
-      Shared& to = ctas == 1 ? sh : *cluster.map_shared_rank(&sh, 0);
+      const uint32_t any = __reduce_or_sync(kFull, where);
 #pragma unroll 1
       for (int it = 0; it < iters; ++it) {
-        if ((where >> (it & 31) & 1u) == 0) continue;
+        if ((any >> (it & 31) & 1u) == 0) continue;
         float v[8];
-        row.load(has ? chunk(it) : row.chunks, v);
+        row.load(where >> (it & 31) & 1u ? chunk(it) : row.chunks, v);
         uint32_t mine = 0;
 #pragma unroll
         for (int j = 0; j < 8; ++j) mine += key_of(v[j]) >= bound ? 1u : 0u;
@@ -583,21 +556,26 @@ struct Sampler {
           const uint32_t c = __shfl_up_sync(kFull, inc, o);
           if (lane >= o) inc += c;
         }
-        uint32_t at = before + inc - mine;
-        before += __shfl_sync(kFull, inc, 31);
+        uint32_t at = 0;
+        if (lane == 31 && inc > 0) at = atomicAdd(&to.listed, inc);
+        at = __shfl_sync(kFull, at, 31);
+        if (at > kList) break;                   // too many, whatever follows
+        at += inc - mine;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           const uint32_t k = key_of(v[j]);
           if (k >= bound) {
-            to.key[at] = k;
-            to.idx[at] = static_cast<uint32_t>(row.index(chunk(it), j));
+            if (at < kList) {
+              to.key[at] = k;
+              to.idx[at] = static_cast<uint32_t>(row.index(chunk(it), j));
+            }
             ++at;
           }
         }
       }
     }
     sync();
-    return all;
+    return to.listed;
   }
 
   // inclusive sum over the threads of the block before and with this one, in a fixed order; only the first `used` warps
@@ -625,18 +603,20 @@ struct Sampler {
     const int t = threadIdx.x, used = (n + 31) / 32;
     const bool have = t < n;
     if (warp < used) {
-      const uint32_t key = have ? sh.key[t] : 0u;
+      const uint32_t key = have ? sh.key[t] : 0u, idx = have ? sh.idx[t] : 0u;
       const double w = weight(have ? value_of(key) : -INFINITY);
-      // rank in descending order; the list is in index order, so ties are won by the earlier position
-      int rank_k = 0;
+      // ranks in descending order (ties are won by the lower index) and by index
+      int rank_k = 0, rank_i = 0;
 #pragma unroll 4
       for (int j = 0; j < n; ++j) {
-        const uint32_t o = sh.key[j];
-        rank_k += (o > key || (o == key && j < t)) ? 1 : 0;
+        const uint32_t o = sh.key[j], i = sh.idx[j];
+        rank_i += i < idx ? 1 : 0;
+        rank_k += (o > key || (o == key && i < idx)) ? 1 : 0;
       }
       if (have) {
-        sh.by_key[rank_k] = static_cast<uint32_t>(t);
-        sh.w[t] = w;
+        sh.by_key[rank_k] = static_cast<uint32_t>(rank_i);
+        sh.w[rank_i] = w;
+        sh.by_idx[rank_i] = idx;
       }
     }
     __syncthreads();
@@ -671,7 +651,7 @@ struct Sampler {
       for (int i = 0; i < used; ++i) {
         if (sh.count[i] == 0) continue;
         const int at = 32 * i + __ffs(sh.count[i]) - 1;
-        write(n_row, static_cast<int>(sh.idx[at]), sh.w[at], total);
+        write(n_row, static_cast<int>(sh.by_idx[at]), sh.w[at], total);
         break;
       }
     }
@@ -774,6 +754,7 @@ struct Sampler {
   }
 
   __device__ __forceinline__ void run(int64_t n) {
+    if (threadIdx.x == 0) sh.listed = 0;
     uint32_t thread_key = largest();
     uint32_t kmax = row_max(thread_key, &Shared::best);
     const float t = p.temperature != nullptr ? p.temperature[n] : p.temperature_all;
@@ -806,16 +787,18 @@ struct Sampler {
     double z = 0.0;
     const Kept all{Cut{0, 0}, 0.0};
     if (k > 0) {
-      if (k <= kThreads) low = max(bound_of_k(thread_key, k), 1u);
+      // a CTA's own: what is among the first k of the row is among the first k of its slice
+      if (k <= kThreads) low = bound_of_k(thread_key, k);
     } else if (by_p) {
       z = sums<kAll>(all, 0);
       low = bound_of_weight((1.0 - share) * z / p.V);
       // that bound is far too low for a steep distribution: try what about kGuess elements reach, and see whether they
       // weigh enough
-      guess = bound_of_k(thread_key, kGuess / ctas);
+      guess = shared_bound(bound_of_k(thread_key, kGuess / ctas));
     }
     if (min_w > 0.0 && !(k > 0 && by_p)) low = max(low, bound_of_weight(min_w));
-    if (low > 1 || guess > 1 || p.V <= kList) {
+    // (decided alike by the CTAs of a row, which wait for one another in there)
+    if ((k > 0 ? k <= kThreads : low > 1 || guess > 1) || p.V <= kList) {
       const bool sure = guess <= low;
       const uint32_t c = gather(max(low, guess), thread_key);
       if (c <= kList) {
