@@ -17,8 +17,12 @@
 //
 // Tokens are decided by comparing sums over the whole vocabulary, so weights are evaluated to 2^-48 in 64 bits and
 // summed in 64 bits: histograms as integers in a fixed point that leaves room for V weights of 1, the rest in floating
-// point in a fixed order. Bound by the 64-bit exponential (11 operations at 60 a clock and SM) where every weight is
-// needed, else by reading the logits.
+// point in a fixed order.
+//
+// Measured (B200): 64 rows of 100,288 bf16 logits, top-k and top-p, 22 us (0.6 TB/s; the read itself takes 2); 256 rows
+// without a filter 74 us, bound by the 64-bit exponentials (47 instructions a logit, 12 of them 64-bit at 60 a clock and
+// SM); one row with top-p 18 us, bound by cluster barriers (1.5 us each) and latency. CTAs a row at 64 rows: 1 / 2 / 4 / 8
+// take 29 / 24 / 22 / 53 us, at one row 53 / 37 / 26 / 18 us, at 400 rows 62 us with one and 152 with two.
 #include <ATen/ATen.h>
 #include <c10/util/Optional.h>
 #include <cooperative_groups.h>

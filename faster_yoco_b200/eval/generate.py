@@ -29,8 +29,8 @@ def generate(model, prompt: torch.Tensor, tokenizer, generate_tokens: int = 20, 
     """prompt: [B, P] ids on the model's device -> [B * num_samples, P + generate_tokens] (pad where nothing was
     produced); rows b * num_samples .. (b + 1) * num_samples - 1 continue prompt b. temperature 0 is greedy; top_k,
     top_p and min_p as in ``ops.sample``; generator: source of its uniform numbers (on the model's device)."""
-    if num_samples < 1:
-        raise ValueError(f"generate: num_samples = {num_samples}")
+    if num_samples < 1 or not temperature >= 0:
+        raise ValueError(f"generate: num_samples = {num_samples}, temperature = {temperature}")
     fork = num_samples > 1 and yoco and hasattr(model, "fork_state")
     if num_samples > 1 and not fork:
         prompt = prompt.repeat_interleave(num_samples, 0)

@@ -607,7 +607,8 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0, top_
     Each of temperature, top_k, top_p and min_p is a number for all rows or a tensor [...] of one for each row (fp32;
     top_k int32 or int64) on the logits' device; numbers are used as fp32. Returns int64 tokens [...], and with
     ``return_logprob`` also the fp32 log-probability of each token under the distribution it was drawn from. Weights
-    and their sums are held in 64 bits, so tokens do not depend on how the work is divided."""
+    and their sums are held in 64 bits: a token differs from the definition's only where u falls within about 1e-10 of a
+    border between two. u = 0 gives the first index of any weight. No gradient."""
     _no_grad_op("sample", logits)
     native = native_on(logits)
     numbers = []

@@ -236,6 +236,8 @@ def test_fork_state_refuses_misuse():
     m, tok = _tiny(), ByteTokenizer()
     with pytest.raises(ValueError):
         generate(m, torch.tensor([[1, 2]]), tok, num_samples=0)
+    with pytest.raises(ValueError):
+        generate(m, torch.tensor([[1, 2]]), tok, temperature=-0.5)
     state = {}
     with torch.no_grad():
         m(torch.tensor([[5, 6, 7]]), incremental_state=state, start_pos=0, is_prefilling=True, skip_cross_decoder=True)
