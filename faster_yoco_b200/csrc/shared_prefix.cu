@@ -23,12 +23,12 @@
 // Work comes in three classes: (0) prefix blocks in pairs, both streams on the same K / V tile (compute bound: halves
 // the shared memory fills); (1) the odd last prefix block, each stream with tiles of its own; (2) own keys.
 //
-// Measured (B200, both kernels, bf16, 24 / 8 heads of 128): 32 rows on 16,384 shared keys with up to 256 of their own 39 us
-// (2.4 TB/s of what has to be read; the floor by bytes is 14), 128 rows on 32,768 + 512 138 us (378 TFLOP/s; floor 52), 20
+// Measured (B200, both kernels, bf16, 24 / 8 heads of 128): 32 rows on 16,384 shared keys with up to 256 of their own 37 us
+// (2.5 TB/s of what has to be read; the floor by bytes is 14), 128 rows on 32,768 + 512 138 us (378 TFLOP/s; floor 52), 20
 // x 24 queries on 2,000 + 24 40 us. What bounds it is neither memory nor the tensor cores (15 % busy) but the chain of a
 // tile: about 2,000 cycles of softmax (exponentials 1,024 at the rate of the SFUs, the rest latency of warps that run
 // alone) and 1,500 of products and hand-over, 4,800 a pair of tiles with two streams. Tried without gain: two threads a
-// row, an issuing warp for each stream, one pass over S, turns at the exponentials, rows of 64 or 128 columns in registers
+// row, four threads a row by copies of short blocks, an issuing warp for each stream, one pass over S, turns at the exponentials, rows of 64 or 128 columns in registers
 // (longer code: slower), launching the join ahead.
 #include <ATen/ATen.h>
 #include <c10/util/Optional.h>
@@ -608,13 +608,14 @@ __global__ void __launch_bounds__(kSpaThreads, 1)
 }
 
 // Joins the pieces of each output row: o = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i. A block has eight consecutive
-// rows of a (group, key / value head): its warps share them out by columns (kJoinCols) and by pieces (Parts), a lane
-// has one row and D / 32 columns in fours, so that a load of a warp covers whole 128-byte lines and a thread has its loads
-// in flight together; the parts join in shared memory.
-template <typename T, int D, int Parts>
+// rows of a (group, key / value head) and 1 / Split of their columns. Its warps share them out by columns (kJoinCols) and by
+// pieces (Parts); a lane has one row and some columns in fours, so that a load of a warp covers whole 128-byte lines and a
+// thread has its loads in flight together; the parts join in shared memory.
+template <typename T, int D, int Parts, int Split>
 __global__ void __launch_bounds__(kJoinCols * Parts * 32) spa_join_kernel(const __grid_constant__ PrefixParams p) {
-  constexpr int F = D / 4 / (4 * kJoinCols);             // float4s of a lane: columns 4 (lane / 8 + 4 (wc + kJoinCols f))
-  __shared__ float4 sO[Parts - 1][D / 4][8];
+  constexpr int F = D / 4 / Split / (4 * kJoinCols);     // float4s of a lane: from c0 on, lane / 8 + 4 (wc + kJoinCols f)
+  const int c0 = static_cast<int>(blockIdx.y) * (D / 4 / Split);
+  __shared__ float4 sO[Parts - 1][D / 4 / Split][8];
   __shared__ float2 sML[Parts][8];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int wc = warp % kJoinCols, wp = warp / kJoinCols;
@@ -633,7 +634,7 @@ __global__ void __launch_bounds__(kJoinCols * Parts * 32) spa_join_kernel(const 
     const float2 ml = *stat;
     float4 t[F];
 #pragma unroll
-    for (int f = 0; f < F; ++f) t[f] = src[((lane >> 3) + 4 * (wc + kJoinCols * f)) * rows];
+    for (int f = 0; f < F; ++f) t[f] = src[(c0 + (lane >> 3) + 4 * (wc + kJoinCols * f)) * rows];
     const bool any = ml.y > 0.f;
     const float Mn = any ? fmaxf(M, ml.x) : M;
     const float f0 = M == -INFINITY ? 0.f : fast_exp2(M - Mn), w = any ? fast_exp2(ml.x - Mn) : 0.f;
@@ -704,7 +705,7 @@ __global__ void __launch_bounds__(kJoinCols * Parts * 32) spa_join_kernel(const 
       const float4 t = sO[q - 1][c4][lane & 7];
       x = make_float4(x.x + w[q] * t.x, x.y + w[q] * t.y, x.z + w[q] * t.z, x.w + w[q] * t.w);
     }
-    *reinterpret_cast<uint2*>(out + 4 * c4) = make_uint2(pack2<T>(x.x * inv, x.y * inv), pack2<T>(x.z * inv, x.w * inv));
+    *reinterpret_cast<uint2*>(out + 4 * (c0 + c4)) = make_uint2(pack2<T>(x.x * inv, x.y * inv), pack2<T>(x.z * inv, x.w * inv));
   }
 }
 
@@ -765,10 +766,15 @@ void launch(const CUtensorMap& pk, const CUtensorMap& pv, const CUtensorMap& k, 
   // pieces of a row, about: ranges that meet a prefix block and those of its own keys
   const int segs = p.G * p.Hk * std::max(p.pairs, 1);
   const int pieces = (p.pairs > 0 ? p.cuts[0].units : p.cuts[1].units) / segs + 2;
-  if (pieces > 8)
-    spa_join_kernel<T, D, 4><<<groups, kJoinCols * 4 * 32, 0, cur_stream()>>>(p);
+  // Few blocks and many pieces: twice the blocks, each with half of the columns, and twice the warps on the pieces (both
+  // kernels, us, with and without: 96 blocks of 39 pieces 37.4 and 40.3; 384 blocks of 20 pieces 144.7 and 137.8; 128
+  // blocks of 11 pieces 52.2 and 49.9). With few pieces two warps share them.
+  if (pieces > 16 && groups < 2 * p.ctas)
+    spa_join_kernel<T, D, 8, 2><<<dim3(groups, 2), kJoinCols * 8 * 32, 0, cur_stream()>>>(p);
+  else if (pieces > 8)
+    spa_join_kernel<T, D, 4, 1><<<groups, kJoinCols * 4 * 32, 0, cur_stream()>>>(p);
   else
-    spa_join_kernel<T, D, 2><<<groups, kJoinCols * 2 * 32, 0, cur_stream()>>>(p);
+    spa_join_kernel<T, D, 2, 1><<<groups, kJoinCols * 2 * 32, 0, cur_stream()>>>(p);
   check_launch("shared_prefix_attention (join)");
 }
 
