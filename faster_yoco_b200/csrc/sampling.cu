@@ -84,19 +84,22 @@ __device__ __forceinline__ float value_of(uint32_t k) {
 // below 2^-48. The table lies in the lanes of the warp (lane j: 2^(j / 32)) and is read by shuffles: all lanes call.
 struct Weight {
   double top, scale, table;  // largest logit (finite), 32 log2(e) / T, this lane's 2^(lane / 32)
-  float topf, scalef, offset;  // in 32 bits; estimate of t: x scalef + offset
+  float half, lowest;        // -max / 2; the (x - max) / 2 of a weight of 2^-1000
   uint32_t kmax;
 
   __device__ __forceinline__ void init(uint32_t largest, float t) {
     kmax = largest;
-    topf = value_of(largest);
+    const float topf = value_of(largest);
     top = static_cast<double>(topf);
     scale = 46.166241308446828384 / static_cast<double>(t);
-    scalef = static_cast<float>(scale);
-    offset = -topf * scalef;
+    half = -0.5f * topf;
+    lowest = fmaxf(static_cast<float>(-16000.0 / scale), -3.402823466e38f);
   }
-  // whether a logit has a weight: not -inf or NaN (the estimate is NaN, which compares as false), not below 2^-1000
-  __device__ __forceinline__ bool some(float x) const { return fmaf(x, scalef, offset) > -32000.0f || x == topf; }
+  // whether a logit has a weight: not -inf or NaN, not below 2^-1000. It goes by the difference of the logits, halved so
+  // that it stays finite: one rounding of what value() evaluates, so that neighbours of the largest are told apart at
+  // any temperature (x scale - max scale in 32 bits is off by thousands where max / T is large, and the exponent field
+  // of a weight below 2^-1022 wraps).
+  __device__ __forceinline__ bool some(float x) const { return fmaf(x, 0.5f, half) >= lowest; }
   // weight of a logit that has one, exactly 1 for the largest; anything for others
   __device__ __forceinline__ double value(float x) const {
     constexpr double kRound = 6755399441055744.0;        // 1.5 x 2^52: adding it rounds to an integer

@@ -111,6 +111,60 @@ def test_sample_edges(V, dtype):
             assert tok[:2].tolist() == [-1, -1] and int(tok[2]) == V - 1 and int(tok[4]) == V // 2
 
 
+@pytest.mark.parametrize("N,V", [(24, 40), (12, 700), (1, 50001), (200, 9001)])
+def test_sample_neighbours_at_low_temperatures(N, V):
+    """Logits a few steps of fp32 below the largest, at temperatures where such a step is anything from nothing to
+    thousands in the exponent: every weight is the definition's, or zero."""
+    g = torch.Generator(device="cuda").manual_seed(V)
+    r = torch.arange(N, device="cuda")
+    top = 120 * torch.rand(N, 1, generator=g, device="cuda") - 60
+    x = top - 0.5 - 5 * torch.rand(N, V, generator=g, device="cuda")
+    at = torch.rand(N, V, generator=g, device="cuda").topk(20, dim=1).indices
+    steps = torch.randint(1, 65, (N, 20), generator=g, device="cuda", dtype=torch.int32)
+    steps[:, 0] = 0
+    # one step down: the next smaller integer image of a positive float, the next larger one of a negative
+    x.scatter_(1, at, (top.view(torch.int32) - steps * top.sign().int()).view(torch.float32))
+    t = torch.tensor([1e-6, 1e-7, 3e-8, 1e-8, 5e-9, 1e-9, 1e-10, 1e-12, 1e-30, 1e-40], device="cuda")[r % 10]
+    for u0 in (0.0, 0.4, 0.8, 1.0 - 2.0 ** -24):
+        u = torch.full((N,), u0, device="cuda")
+        for kw in (dict(), dict(k=10), dict(p=0.7), dict(mp=0.3), dict(k=600, p=0.9)):
+            check_sample(x, u, t, **kw)
+
+
+def check_sample_on_borders(x, u, t=1.0, k=0, p=1.0, mp=0.0):
+    """check_sample for rows where u may fall ON a border between two tokens (a pattern that repeats, halved by u = 0.5:
+    the first half of 900 logits of weights 1, w, w, 1, w, w, ... is exactly half of them, so the rounding of the sums says
+    which side of it a token lies). Sums of at most 2^17 weights, each within 2^-48, in 64 bits are within 2^17 2^-53 +
+    2^-48 < 2^-34 of their value: the token is the definition's at u (1 - 2^-34) or at u (1 + 2^-34)."""
+    N = x.shape[0]
+    tok, lp = ops.sample(x, u, t, k, p, mp, return_logprob=True)
+    pars = (rows_of(t, N, torch.float32), rows_of(k, N, torch.int64), rows_of(p, N, torch.float32),
+            rows_of(mp, N, torch.float32))
+    good = torch.zeros(N, dtype=torch.bool, device="cuda")
+    for side in (1 - 2.0 ** -34, 1 + 2.0 ** -34):
+        want, wlp = ref.sample(x, u.double() * side, *pars)
+        tol = 2.0 ** -23 * wlp.abs() + 2.0 ** -28
+        good |= (tok == want) & ((lp.double() - wlp.double()).abs() <= tol)
+    assert bool(good.all())
+
+
+@pytest.mark.parametrize("V", [8, 900, 40000])
+def test_sample_largest_far_below_zero(V):
+    low = torch.finfo(torch.float32).min
+    x = torch.full((6, V), low, device="cuda")
+    x[0, V // 2] = -1e38
+    x[1, ::3] = -2e38
+    x[2, 1::2] = -3e38
+    x[3] = torch.linspace(-1e37, -3.4e38, V, device="cuda")
+    x[4] = -10 - torch.arange(V, device="cuda") / V
+    x[5, 2:5] = 3e38
+    for u0 in (0.0, 0.5, 1.0 - 2.0 ** -24):
+        u = torch.full((6,), u0, device="cuda")
+        for t in (1.0, 1e-36, 1e38, 3e38):
+            for kw in (dict(), dict(k=4), dict(p=0.6), dict(mp=0.5), dict(k=700, p=0.9)):
+                check_sample_on_borders(x, u, t, **kw)
+
+
 def test_sample_row_parameters():
     N, V = 60, 30011
     x = logits_like(N, V, torch.bfloat16, seed=3)
