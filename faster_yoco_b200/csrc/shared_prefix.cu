@@ -635,7 +635,7 @@ __global__ void __launch_bounds__(kJoinCols * Parts * 32) spa_join_kernel(const 
     float4 t[F];
 #pragma unroll
     for (int f = 0; f < F; ++f) t[f] = src[(c0 + (lane >> 3) + 4 * (wc + kJoinCols * f)) * rows];
-    const bool any = ml.y > 0.f;
+    const bool any = ml.y != 0.f;            // a NaN score has to reach the result: its piece's sum is NaN
     const float Mn = any ? fmaxf(M, ml.x) : M;
     const float f0 = M == -INFINITY ? 0.f : fast_exp2(M - Mn), w = any ? fast_exp2(ml.x - Mn) : 0.f;
     M = Mn;
@@ -691,10 +691,10 @@ __global__ void __launch_bounds__(kJoinCols * Parts * 32) spa_join_kernel(const 
 #pragma unroll
   for (int q = 0; q < Parts; ++q) {
     const float2 ml = sML[q][lane & 7];
-    w[q] = ml.y > 0.f ? fast_exp2(ml.x - top) : 0.f;
+    w[q] = ml.y != 0.f ? fast_exp2(ml.x - top) : 0.f;
     total += w[q] * ml.y;
   }
-  const float inv = total > 0.f ? 1.0f / total : 0.f;
+  const float inv = total != 0.f ? 1.0f / total : 0.f;       // no key seen: zeros; a NaN stays one
   T* out = reinterpret_cast<T*>(p.o) + ((static_cast<int64_t>(b) * p.Lq + i) * p.Hq + hk * p.rep + hr) * D;
 #pragma unroll
   for (int f = 0; f < F; ++f) {

@@ -553,8 +553,10 @@ def shared_prefix_attention(q: torch.Tensor, prefix_k: torch.Tensor, prefix_v: t
     means all stored positions. Positions behind the lengths may hold anything. P, S, B or Lq may be 0; a query that
     sees no key gets zeros. scale: default 1 / sqrt(D). Returns a contiguous [B, Lq, Hq, D].
 
-    The sm_100a kernel takes bf16 and fp16 with D 64 or 128; other types and sizes run the PyTorch expression. Key / value tensors are read in place when their rows are 16-byte
-    aligned, else copied first. A value that SOME query of a row sees has to be finite. Inference only."""
+    The sm_100a kernel takes bf16 and fp16 with D 64 or 128; other types and sizes run the PyTorch expression. Key / value
+    tensors are read in place when their rows are 16-byte aligned, else copied first. A NaN in a query, or in a key that it
+    sees, makes its result NaN (as does a score of +inf). A value that SOME query of a row sees has to be finite.
+    Inference only."""
     _no_grad_op("shared_prefix_attention", q, prefix_k, prefix_v, k, v)
     scale = max(q.shape[-1], 1) ** -0.5 if scale is None else float(scale)
     if not 0.0 < scale < math.inf:

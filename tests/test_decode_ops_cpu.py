@@ -154,6 +154,27 @@ def test_shared_prefix_equals_attention():
     torch.testing.assert_close(got, want, rtol=1e-5, atol=1e-5)
 
 
+def test_shared_prefix_nan_reaches_the_result():
+    """A NaN query, and a NaN or +inf score among those that a query sees, give NaN; all other results stay as they are."""
+    gen = torch.Generator().manual_seed(9)
+    r = lambda *s: torch.randn(*s, generator=gen)
+    q, pk, pv, k, v = r(4, 3, 4, 16), r(2, 9, 2, 16), r(2, 9, 2, 16), r(4, 5, 2, 16), r(4, 5, 2, 16)
+    want = ops.shared_prefix_attention(q, pk, pv, k, v)
+    bad = torch.zeros(4, 3, 4, dtype=torch.bool)
+    q[0, 1, 2, 5] = float("nan")
+    bad[0, 1, 2] = True
+    pk[1, 4, 1, 0] = float("nan")              # rows 2 and 3, the second key / value head's query heads
+    bad[2:, :, 2:] = True
+    k[1, 3, 0, 7] = float("nan")               # own key 3 of 5: of three queries the last two see it
+    bad[1, 1:, :2] = True
+    k[3, 0, 0] = INF * q[3, 0, 0].sign()       # a score of +inf for one query, of mixed signs (NaN) for the others
+    bad[3, :, 1] = torch.isnan(q[3, :, 1] @ k[3, 0, 0]) | ((q[3, :, 1] @ k[3, 0, 0]) == INF)
+    bad[3, :, 0] = True
+    got = ops.shared_prefix_attention(q, pk, pv, k, v)
+    assert torch.equal(torch.isnan(got).all(-1), bad) and torch.equal(torch.isnan(got).any(-1), bad)
+    torch.testing.assert_close(got[~bad], want[~bad], rtol=1e-6, atol=1e-6)
+
+
 def test_shared_prefix_refusals():
     r = torch.randn
     q, pk, k = r(4, 1, 4, 16), r(2, 5, 2, 16), r(4, 3, 2, 16)

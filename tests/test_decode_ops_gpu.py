@@ -358,6 +358,30 @@ def test_shared_prefix_scores_far_apart():
         check_attention(x, lengths, pre, scale=0.3)
 
 
+@pytest.mark.parametrize("G,n,Lq,P,S", [(2, 3, 1, 40, 9), (2, 20, 1, 3000, 300), (2, 70, 1, 900, 140), (2, 4, 5, 2000, 200)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_shared_prefix_nan_reaches_the_result(G, n, Lq, P, S, dtype):
+    """One NaN in a query, in a prefix key or in an own key makes the results that see it NaN, wherever the keys are cut
+    into pieces, and leaves the bits of all others as they are. The PyTorch form says the same."""
+    x, lengths, pre = make(G, n, Lq, 6, 2, 128, P, S, dtype, False)
+    want = ops.shared_prefix_attention(*x.values(), lengths=lengths, prefix_lengths=pre)
+    spots = {"q": (1, 0, 2, 7), "pk": (1, P - 5, 1, 3), "k": (0, S - Lq, 0, 127)}
+    seen = {"q": (1, 0, 2), "pk": (slice(n, None), slice(None), slice(3, None)), "k": (0, slice(None), slice(0, 3))}
+    for name, at in spots.items():
+        for value in ((float("nan"), INF) if name == "q" else (float("nan"),)):
+            y = {a: t.clone() for a, t in x.items()}
+            y[name][at] = value
+            bad = torch.zeros(want.shape[:3], dtype=torch.bool, device="cuda")
+            bad[seen[name]] = True
+            for backend in ("native", "torch"):
+                ops.set_backend(backend)
+                got = ops.shared_prefix_attention(*y.values(), lengths=lengths, prefix_lengths=pre)
+                ops.set_backend("native")
+                assert torch.equal(torch.isnan(got).all(-1), bad) and torch.equal(torch.isnan(got).any(-1), bad)
+                if backend == "native":
+                    assert torch.equal(got[~bad], want[~bad])
+
+
 def test_shared_prefix_other_types():
     """fp32 and other head dims take the PyTorch expression."""
     for dtype, D in ((torch.float32, 128), (torch.float16, 32)):
