@@ -35,6 +35,7 @@
 #include <cuda_fp16.h>
 
 #include <atomic>
+#include <cmath>
 
 #include "common/host.h"
 #include "common/ptx.cuh"
@@ -788,7 +789,10 @@ at::Tensor shared_prefix_attention(const at::Tensor& q, const at::Tensor& pk, co
   FYB_SUITS(q.is_cuda() && q.dim() == 4 && (q.size(3) == 64 || q.size(3) == 128) &&
                 (q.scalar_type() == at::kBFloat16 || q.scalar_type() == at::kHalf),
             "shared_prefix_attention: bf16 or fp16 q [B, Lq, Hq, 64 or 128] expected");
-  FYB_SUITS(scale > 0 && std::isfinite(scale), "shared_prefix_attention: scale must be positive");
+  // as the kernel holds it: a factor of zero would make NaN of the -inf of hidden keys
+  const float scale_log2 = static_cast<float>(scale * 1.4426950408889634);
+  FYB_SUITS(std::isnormal(scale_log2) && scale_log2 > 0,
+            "shared_prefix_attention: scale must be positive and within fp32");
   const int64_t B = q.size(0), Lq = q.size(1), Hq = q.size(2), D = q.size(3);
   PrefixParams p{};
   p.q = view_of(q, q, "q");
@@ -829,7 +833,7 @@ at::Tensor shared_prefix_attention(const at::Tensor& q, const at::Tensor& pk, co
   p.shift = p.cuts[1].units % (2 * p.ctas);
   p.lengths = length_ptr(lengths, q, B, p.lengths_64);
   p.prefix_lengths = length_ptr(prefix_lengths, q, G, p.prefix_lengths_64);
-  p.scale_log2 = (float)(scale * 1.4426950408889634);
+  p.scale_log2 = scale_log2;
   p.o = o.data_ptr();
   p.status = status_ptr();
   // a slot for each (range, block) that can meet: ranges + blocks, as both only move forward

@@ -551,12 +551,12 @@ def shared_prefix_attention(q: torch.Tensor, prefix_k: torch.Tensor, prefix_v: t
     own keys j < lengths[b] with j <= lengths[b] - Lq + i (the causal diagonal ends at the last own key, as in
     ``attention``). lengths [B] / prefix_lengths [G]: int32 or int64 on q's device, clamped to [0, S] / [0, P]; None
     means all stored positions. Positions behind the lengths may hold anything. P, S, B or Lq may be 0; a query that
-    sees no key gets zeros. scale: default 1 / sqrt(D). Returns a contiguous [B, Lq, Hq, D].
+    sees no key gets zeros. scale: positive, default 1 / sqrt(D). Returns a contiguous [B, Lq, Hq, D].
 
-    The sm_100a kernel takes bf16 and fp16 with D 64 or 128; other types and sizes run the PyTorch expression. Key / value
-    tensors are read in place when their rows are 16-byte aligned, else copied first. A NaN in a query, or in a key that it
-    sees, makes its result NaN (as does a score of +inf). A value that SOME query of a row sees has to be finite.
-    Inference only."""
+    The sm_100a kernel takes bf16 and fp16 with D 64 or 128 (and refuses a scale that is not normal in fp32); other types
+    and sizes run the PyTorch expression. Key / value tensors are read in place when their rows are 16-byte aligned, else
+    copied first. A NaN in a query, or in a key that it sees, makes its result NaN (as does a score of +inf). A value that SOME query of a
+    row sees has to be finite. Inference only."""
     _no_grad_op("shared_prefix_attention", q, prefix_k, prefix_v, k, v)
     scale = max(q.shape[-1], 1) ** -0.5 if scale is None else float(scale)
     if not 0.0 < scale < math.inf:
@@ -585,6 +585,8 @@ def shared_prefix_attention(q: torch.Tensor, prefix_k: torch.Tensor, prefix_v: t
         if t is not None and (t.shape != (m,) or t.dtype not in (torch.int32, torch.int64) or t.device != q.device):
             raise ValueError(f"shared_prefix_attention: {what} must be int32 or int64 [{m}] on {q.device}")
     if native and q.dtype in (torch.bfloat16, torch.float16) and D in (64, 128):
+        if not torch.finfo(torch.float32).tiny <= scale / math.log(2) <= torch.finfo(torch.float32).max:
+            raise ValueError(f"shared_prefix_attention: scale = {scale} is not within fp32")
         lengths, prefix_lengths = (t if t is None else t.contiguous() for t in (lengths, prefix_lengths))
         return _C().shared_prefix_attention(_vec16(q), *(_vec16(t) for t in kv), lengths, prefix_lengths, scale)
     return ref.shared_prefix_attention(q, *kv, lengths, prefix_lengths, scale)

@@ -468,6 +468,22 @@ def test_native_refusals():
         ops.shared_prefix_attention(q, pk, pv, k, v, lengths=lengths.cpu())
 
 
+@pytest.mark.parametrize("scale", [1e-46, 1e-39, 1e39, 1e300])
+def test_shared_prefix_refuses_scales_outside_fp32(scale):
+    """Zero or infinite as an fp32 factor: hidden keys' -inf would become NaN."""
+    x, lengths, pre = make(1, 4, 1, 6, 2, 128, 20, 5, torch.bfloat16, True)
+    with pytest.raises(RuntimeError):
+        ops._C().shared_prefix_attention(*x.values(), lengths, pre, scale)
+    with pytest.raises(ValueError):
+        ops.shared_prefix_attention(*x.values(), lengths=lengths, prefix_lengths=pre, scale=scale)
+
+
+@pytest.mark.parametrize("scale", [2.0 ** -126, 1e-30, 1e-3])
+def test_shared_prefix_small_scales(scale):
+    x, lengths, pre = make(2, 4, 1, 6, 2, 128, 200, 50, torch.bfloat16, True)
+    check_attention(x, lengths, pre, scale=scale)
+
+
 # ----------------------------------------------------------------------------------------------------------------------
 # the run of them that generation makes
 
