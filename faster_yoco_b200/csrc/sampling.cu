@@ -16,8 +16,8 @@
 //   counts (top-k) or weights (top-p) in steps of 11 bits, and the draw goes by segment sums.
 //
 // Tokens are decided by comparing sums over the whole vocabulary, so weights are evaluated to 2^-48 in 64 bits and
-// summed in 64 bits: histograms as integers in a fixed point that leaves room for V weights of 1, the rest in floating
-// point in a fixed order.
+// summed in 64 bits: histograms as integers in a fixed point whose 62 bits the weight of all candidates fills, the rest in
+// floating point in a fixed order.
 //
 // Measured (B200): 64 rows of 100,288 bf16 logits, top-k and top-p, 22 us (0.6 TB/s; the read itself takes 2); 256 rows
 // without a filter 74 us, bound by the 64-bit exponentials (47 instructions a logit, 12 of them 64-bit at 60 a clock and
@@ -58,7 +58,6 @@ struct SampleParams {
   float temperature_all, top_p_all, min_p_all;
   int64_t top_k_all;
   int top_k_64;
-  double unit;               // fixed-point units of a weight of 1
   int64_t* token;
   float* logprob;            // or null
 };
@@ -227,7 +226,6 @@ struct Shared {
   uint32_t warp_best[kWarps];
   uint32_t best, first;                // of this CTA: largest image; ~(lowest index that has the row's largest)
   uint32_t bound;                      // of this CTA
-  uint64_t weight;                     // of this CTA, in fixed point
   double part[kWarps][kGranules];      // weight of each granule
   double part_sum[kWarps];
   double sum;                          // of this CTA
@@ -256,6 +254,7 @@ struct Sampler {
   Weight weight;
   int rank, ctas, warp, lane;
   int c0, c1, per, iters, step;        // this warp's chunks; chunks and iterations a warp, iterations of a granule
+  double unit = 1.0;                   // fixed-point units of a weight of 1
 
   __device__ __forceinline__ Sampler(const SampleParams& p_, Shared& s, int64_t n)
       : p(p_), sh(s), cluster(cg::this_cluster()), row(p_, n) {
@@ -665,7 +664,13 @@ struct Sampler {
     return true;
   }
 
-  __device__ __forceinline__ uint64_t fixed(double w) const { return static_cast<uint64_t>(__double2ll_rn(w * p.unit)); }
+  __device__ __forceinline__ uint64_t fixed(double w) const { return static_cast<uint64_t>(__double2ll_rn(w * unit)); }
+  // a unit in which weights of `total` (1 or more) together take 62 bits: what V of them lose by rounding is below 2^-62 V of
+  // the total, however many the small ones are (V weights of 1 would leave 2^-40 for one of 2^22 logits)
+  __device__ __forceinline__ void set_unit(double total) {
+    const int e = (__double2hiint(total) >> 20) - 1022;        // total < 2^e
+    unit = __hiloint2double((1023 + 62 - e) << 20, 0);
+  }
 
   // The image at which the amount of larger and equal images first reaches `target`: 1 for each candidate that the cut
   // keeps, or its fixed-point weight. Steps of kBinBits over the images from `low` (> 0) up, which hold the answer.
@@ -830,29 +835,28 @@ struct Sampler {
       cut = Cut{key, static_cast<uint32_t>(min(left, at))};
     }
     if (by_p) {
-      double kept_weight = z * p.unit;             // in fixed-point units
       if (k > 0) {
-        uint64_t sum = 0;
+        double sum = 0.0;
         for (int it = 0; it < iters; ++it) {
           float v[8];
           row.load(chunk(it), v);
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
-            const uint64_t a = fixed(weight(v[j]));
-            sum += key_of(v[j]) > cut.key ? a : 0;
+            const double w = weight(v[j]);
+            sum += key_of(v[j]) > cut.key ? w : 0.0;
           }
         }
         const double wt = weight(value_of(cut.key));
-        sum = block_scan(sum, sh.scan);
+        sum = block_scan(sum, sh.part_sum);
         __syncthreads();
-        if (threadIdx.x == kThreads - 1) sh.weight = sum;
+        if (threadIdx.x == kThreads - 1) sh.sum = sum;
         sync();
-        sum = cut.ties * fixed(wt);
-        for (int r = 0; r < ctas; ++r) sum += of(r).weight;
-        kept_weight = static_cast<double>(sum);
+        z = cut.ties * wt;
+        for (int r = 0; r < ctas; ++r) z += of(r).sum;
         low = cut.key;
       }
-      const double target = fmax(share * kept_weight, 1.0);      // the largest is always kept
+      set_unit(z);
+      const double target = fmax(share * (z * unit), 1.0);       // the largest is always kept
       const uint32_t key = radix_find<true>(cut, low, target, above, at);
       const uint64_t w = fixed(weight(value_of(key)));
       uint64_t ties = 1;
@@ -951,9 +955,6 @@ std::vector<at::Tensor> sample(const at::Tensor& logits, const at::Tensor& u,
   p.top_p_all = static_cast<float>(top_p_all);
   p.min_p_all = static_cast<float>(min_p_all);
   p.top_k_all = top_k_all;
-  int bits = 0;
-  while ((1ll << bits) < V) ++bits;
-  p.unit = std::ldexp(1.0, 62 - bits);
   auto token = at::empty({N}, logits.options().dtype(at::kLong));
   at::Tensor logprob;
   if (want_logprob) logprob = at::empty({N}, logits.options().dtype(at::kFloat));

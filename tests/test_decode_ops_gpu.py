@@ -165,6 +165,19 @@ def test_sample_largest_far_below_zero(V):
                 check_sample_on_borders(x, u, t, **kw)
 
 
+@pytest.mark.parametrize("kw", [dict(p=1 - 2.0 ** -22), dict(k=(1 << 22) - 3, p=1 - 2.0 ** -22)])
+def test_sample_tail_of_many_small_weights(kw):
+    """2^22 logits: the last one weighs 1, the others about 2^-42 each, 2^-20 together, of which top-p leaves three quarters.
+    Tokens of the tail come before the heavy one, so u well below their share picks one of them, at an index that the
+    rounding of 64-bit sums (2^22 2^-53 of their value) moves by less than a thousandth."""
+    V = 1 << 22
+    x = torch.full((3, V), -42 * math.log(2), device="cuda")
+    x[:, -1] = 0.0
+    u = torch.tensor([2.0 ** -22, 1.7e-7, 0.9], device="cuda")
+    tok = check_sample(x, u, **kw)
+    assert int(tok[0]) < V // 2 and int(tok[2]) == V - 1
+
+
 def test_sample_row_parameters():
     N, V = 60, 30011
     x = logits_like(N, V, torch.bfloat16, seed=3)
