@@ -28,7 +28,8 @@ def generate(model, prompt: torch.Tensor, tokenizer, generate_tokens: int = 20, 
              min_p: float = 0.0, generator: Optional[torch.Generator] = None) -> torch.Tensor:
     """prompt: [B, P] ids on the model's device -> [B * num_samples, P + generate_tokens] (pad where nothing was
     produced); rows b * num_samples .. (b + 1) * num_samples - 1 continue prompt b. temperature 0 is greedy; top_k,
-    top_p and min_p as in ``ops.sample``; generator: source of its uniform numbers (on the model's device)."""
+    top_p and min_p as in ``ops.sample``; generator: source of its uniform numbers (on the model's device). A sampled row
+    whose logits leave nothing to draw (all NaN or -inf) raises RuntimeError."""
     if num_samples < 1 or not temperature >= 0:
         raise ValueError(f"generate: num_samples = {num_samples}, temperature = {temperature}")
     fork = num_samples > 1 and yoco and hasattr(model, "fork_state")
@@ -61,9 +62,15 @@ def generate(model, prompt: torch.Tensor, tokenizer, generate_tokens: int = 20, 
         else:
             nxt = logits.argmax(-1)
         cur = out[:, idx]
-        nxt = torch.where((cur == tokenizer.pad_id) & ~eos, nxt, cur)
+        live = (cur == tokenizer.pad_id) & ~eos
+        stuck = live & (nxt < 0)           # ops.sample's -1: a row without candidates, no token to go on with
+        nxt = torch.where(live, nxt, cur)
         out[:, idx] = nxt
         eos |= nxt == tokenizer.eos_id
-        if bool(eos.all()):
+        ended, failed = torch.stack([eos.all(), stuck.any()]).tolist()
+        if failed:
+            raise RuntimeError(f"generate: no token can be drawn at position {idx} for rows "
+                               f"{stuck.nonzero().flatten().tolist()}: all their logits are NaN or -inf")
+        if ended:
             break
     return out

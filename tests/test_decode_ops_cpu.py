@@ -251,6 +251,40 @@ def test_sampled_generation_of_other_models():
     assert out.shape == (3, prompt.shape[1] + 3)
 
 
+class _Scripted(torch.nn.Module):
+    """A model whose logits at a position are given: [rows, vocabulary] by position."""
+
+    def __init__(self, logits):
+        super().__init__()
+        self.logits = logits
+
+    def forward(self, x, incremental_state=None, start_pos=0, is_prefilling=True, **_):
+        return (None if is_prefilling else self.logits[start_pos][:, None].clone()), None
+
+
+@pytest.mark.parametrize("nothing", [float("nan"), -INF])
+def test_sampled_generation_of_a_row_without_candidates(nothing):
+    """Logits that leave nothing to draw end generation with an error, unless the row has ended before."""
+    from faster_yoco_b200.eval.generate import generate
+    ops.set_backend("torch")
+    tok = ByteTokenizer()
+    prompt = torch.tensor([tok.encode("ab", bos=True)] * 3)
+    P = prompt.shape[1]
+    gen = torch.Generator().manual_seed(0)
+    logits = {P - 1 + i: torch.randn(3, 264, generator=gen) for i in range(4)}
+    logits[P - 1][1] = -INF                    # row 1 ends with its first token
+    logits[P - 1][1, tok.eos_id] = 0.0
+    logits[P - 1][::2, tok.eos_id] = -INF
+    logits[P][1] = nothing
+    logits[P][::2, tok.eos_id] = -INF
+    m = _Scripted(logits)
+    out = generate(m, prompt, tok, generate_tokens=2, temperature=1.0, yoco=False)
+    assert bool((out >= 0).all()) and int(out[1, P]) == tok.eos_id and int(out[1, P + 1]) == tok.pad_id
+    logits[P + 1][2] = nothing
+    with pytest.raises(RuntimeError, match=r"rows \[2\]"):
+        generate(m, prompt, tok, generate_tokens=3, temperature=1.0, yoco=False)
+
+
 def test_fork_state_refuses_misuse():
     from faster_yoco_b200.eval.generate import generate
     ops.set_backend("torch")
