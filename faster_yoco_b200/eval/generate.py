@@ -20,6 +20,7 @@ from typing import Optional
 import torch
 
 from .. import ops
+from ..parallel import tp as TP
 
 
 @torch.no_grad()
@@ -28,8 +29,8 @@ def generate(model, prompt: torch.Tensor, tokenizer, generate_tokens: int = 20, 
              min_p: float = 0.0, generator: Optional[torch.Generator] = None) -> torch.Tensor:
     """prompt: [B, P] ids on the model's device -> [B * num_samples, P + generate_tokens] (pad where nothing was
     produced); rows b * num_samples .. (b + 1) * num_samples - 1 continue prompt b. temperature 0 is greedy; top_k,
-    top_p and min_p as in ``ops.sample``; generator: source of its uniform numbers (on the model's device). A sampled row
-    whose logits leave nothing to draw (all NaN or -inf) raises RuntimeError."""
+    top_p and min_p as in ``ops.sample``; generator: source of its uniform numbers (on the model's device; of tensor-parallel
+    ranks the first one's decide). A sampled row whose logits leave nothing to draw (all NaN or -inf) raises RuntimeError."""
     if num_samples < 1 or not temperature >= 0:
         raise ValueError(f"generate: num_samples = {num_samples}, temperature = {temperature}")
     fork = num_samples > 1 and yoco and hasattr(model, "fork_state")
@@ -58,7 +59,7 @@ def generate(model, prompt: torch.Tensor, tokenizer, generate_tokens: int = 20, 
         logits[:, tokenizer.pad_id] = -math.inf
         if temperature > 0:
             u = torch.rand(logits.shape[0], generator=generator, device=dev)
-            nxt = ops.sample(logits, u, temperature, top_k, top_p, min_p)
+            nxt = TP.from_first_rank(ops.sample(logits, u, temperature, top_k, top_p, min_p))
         else:
             nxt = logits.argmax(-1)
         cur = out[:, idx]

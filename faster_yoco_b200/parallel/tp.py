@@ -103,6 +103,15 @@ def _split_last(x: torch.Tensor) -> torch.Tensor:
     return x[..., _TP_RANK * n:(_TP_RANK + 1) * n].contiguous()
 
 
+def from_first_rank(x: torch.Tensor) -> torch.Tensor:
+    """x of the first rank of the tensor-parallel group, on all its ranks (what each draws for itself would differ)."""
+    if _TP_SIZE == 1 or _TP_GROUP is None:
+        return x
+    x = x.contiguous()
+    dist.broadcast(x, src=dist.get_global_rank(_TP_GROUP, 0), group=_TP_GROUP)
+    return x
+
+
 class _CopyToTP(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x):

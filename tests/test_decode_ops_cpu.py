@@ -301,3 +301,30 @@ def test_fork_state_refuses_misuse():
             m.fork_state(forked, 2, 2)
         with pytest.raises(ValueError):
             m(torch.tensor([[5], [6]]), incremental_state=forked, start_pos=2, is_prefilling=False)
+
+
+def _tp_generation_worker(rank, world, full_sd, prompt, want):
+    from faster_yoco_b200.eval.generate import generate
+    from faster_yoco_b200.models.yoco import YOCO, shard_state_dict
+    from faster_yoco_b200.parallel import tp
+    ops.set_backend("torch")
+    tp.init_model_parallel(world)
+    m = YOCO(build_args("yoco_tiny", vocab_size=264, n_layers=2, max_seq_len=512, max_batch_size=2,
+                        model_parallel_size=world)).eval()
+    m.load_state_dict(shard_state_dict(full_sd, world, rank), strict=True)
+    out = generate(m, prompt, ByteTokenizer(), generate_tokens=8, chunk_length=8, num_samples=3, temperature=1.0, top_p=0.9,
+                   generator=torch.Generator().manual_seed(20 + rank))
+    assert torch.equal(out, want)
+    tp.destroy_model_parallel()
+
+
+def test_sampled_generation_of_tensor_parallel_ranks():
+    """Two ranks whose generators differ go on with the same tokens: those of one rank with the first one's generator."""
+    from faster_yoco_b200.eval.generate import generate
+    from faster_yoco_b200.utils.launch import run_ranks
+    ops.set_backend("torch")
+    m, tok = _tiny(), ByteTokenizer()
+    prompt = torch.tensor([tok.encode("two ranks", bos=True)])
+    want = generate(m, prompt, tok, generate_tokens=8, chunk_length=8, num_samples=3, temperature=1.0, top_p=0.9,
+                    generator=torch.Generator().manual_seed(20))
+    run_ranks(_tp_generation_worker, 2, {k: v.detach().clone() for k, v in m.state_dict().items()}, prompt, want)
