@@ -211,6 +211,10 @@ class CrossDecoder(nn.Module):
                     nk[:, :have] = st["prev_key"]
                     nv[:, :have] = st["prev_value"]
                 st["prev_key"], st["prev_value"] = nk, nv
+                st.pop("lent", None)
+            elif start_pos < st.get("lent", 0):  # forked states read these positions: they keep what they were given
+                st["prev_key"], st["prev_value"] = st["prev_key"].clone(), st["prev_value"].clone()
+                del st["lent"]
             st["prev_key"][:, start_pos:start_pos + seqlen] = key
             st["prev_value"][:, start_pos:start_pos + seqlen] = value
             st["filled"] = start_pos + seqlen
@@ -355,7 +359,8 @@ class YOCO(nn.Module):
         """The incremental state of ``batch * copies`` rows (row r continues prompt r // copies) from the state of
         ``batch`` prefilled prompts: the self-decoder's states, which do not grow with the prompt, are copied; the one
         shared K / V cache of the prompts becomes a prefix that the copies read in place, and each copy gets a cache
-        of its own for the positions after it."""
+        of its own for the positions after it. ``state`` may go on: behind the prompts it shares their cache, and a step
+        that starts inside them moves it to a copy first."""
         out: Dict = {}
         for idx in range(len(self.self_decoder.layers)):
             st = out[idx] = dict(state.get(idx, {}))
@@ -367,6 +372,8 @@ class YOCO(nn.Module):
         if "prefix_key" in state:
             raise ValueError("fork_state: the state is forked already")
         n = state.get("filled", 0)
+        if n:
+            state["lent"] = max(n, state.get("lent", 0))
         for name in ("key", "value"):
             full = state.get("prev_" + name)
             out["prefix_" + name] = (full[:batch, :n] if full is not None else

@@ -251,6 +251,44 @@ def test_sampled_generation_of_other_models():
     assert out.shape == (3, prompt.shape[1] + 3)
 
 
+@pytest.mark.parametrize("window", [None, 16])
+@pytest.mark.parametrize("copies", [1, 3])
+def test_a_forked_state_outlives_what_its_parent_does(window, copies):
+    """The parent goes on behind the prompt, starts again inside it and is overwritten from its first position; states
+    that were forked before each of these decode as if it had rested."""
+    ops.set_backend("torch")
+    m = _tiny(sliding_window=window)
+    gen = torch.Generator().manual_seed(2)
+    prompt, other = (torch.randint(3, 264, (2, 40), generator=gen) for _ in range(2))
+    step = torch.randint(3, 264, (2 * copies, 1), generator=gen)
+
+    def fill(state, ids, at):
+        m(ids, incremental_state=state, start_pos=at, is_prefilling=True, skip_cross_decoder=True)
+
+    def decode(forked):
+        return torch.cat([m(step, incremental_state=forked, start_pos=40 + i, is_prefilling=False)[0] for i in range(2)], 1)
+
+    with torch.no_grad():
+        state = {}
+        fill(state, prompt, 0)
+        want = decode(m.fork_state(state, 2, copies))
+        first, second = m.fork_state(state, 2, copies), m.fork_state(state, 2, copies)
+        cache = state["prev_key"]
+        m(prompt[:, :1], incremental_state=state, start_pos=40, is_prefilling=False)
+        assert state["prev_key"] is cache                  # behind the prompt nothing has to move
+        assert torch.equal(decode(first), want)
+        m(prompt[:, :1], incremental_state=state, start_pos=20, is_prefilling=False)
+        fill(state, other, 0)
+        assert torch.equal(decode(second), want)
+        assert state["prev_key"] is not cache and "lent" not in state
+    long = {}
+    with torch.no_grad():                                  # a cache that grows leaves the lent one behind
+        fill(long, prompt, 0)
+        forked = m.fork_state(long, 2, copies)
+        fill(long, torch.randint(3, 264, (2, 600), generator=gen), 0)
+        assert "lent" not in long and torch.equal(decode(forked), want)
+
+
 class _Scripted(torch.nn.Module):
     """A model whose logits at a position are given: [rows, vocabulary] by position."""
 
