@@ -620,10 +620,11 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0, top_
                             ("top_p", top_p, 0.0, math.inf), ("min_p", min_p, 0.0, 1.0)):
         if isinstance(x, torch.Tensor):
             numbers.append((x, 0))
-        elif lo <= x <= hi:
+        elif lo <= x <= hi and (name != "top_k" or x == int(x)):
             numbers.append((None, min(max(int(x), 0), 1 << 40) if name == "top_k" else float(x)))
         else:
-            raise ValueError(f"sample: {name} = {x} is outside [{lo}, {hi}]")
+            raise ValueError(f"sample: {name} = {x} must be " +
+                             ("a whole number" if name == "top_k" else f"in [{lo}, {hi}]"))
     (t, t1), (k, k1), (p, p1), (m, m1) = numbers
     if native:
         try:

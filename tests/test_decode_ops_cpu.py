@@ -104,6 +104,17 @@ def test_sample_refusals():
         ops.sample(x, u)
 
 
+@pytest.mark.parametrize("top_k", [0.5, 2.7, -0.1, INF, -INF, float("nan")])
+def test_sample_refuses_a_top_k_that_is_no_whole_number(top_k):
+    """0.5 is not the 0 that keeps everything."""
+    x, u = torch.randn(2, 4), torch.rand(2)
+    with pytest.raises(ValueError, match="top_k"):
+        ops.sample(x, u, top_k=top_k)
+    assert torch.equal(ops.sample(x, u, top_k=2.0), ops.sample(x, u, top_k=2))
+    assert torch.equal(ops.sample(x, u, top_k=-(1 << 50)), ops.sample(x, u))
+    assert torch.equal(ops.sample(x, u, top_k=1 << 50), ops.sample(x, u))
+
+
 # ----------------------------------------------------------------------------------------------------------------------
 # shared-prefix attention
 
