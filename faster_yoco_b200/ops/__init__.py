@@ -608,8 +608,8 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0, top_
     than u times the kept weight. temperature <= 0 (or NaN): the largest logit, lowest index first. Several logits of
     +inf share the weight equally. A row without candidates gives token -1 and log-probability -inf.
 
-    Each of temperature, top_k, top_p and min_p is a number for all rows or a tensor [...] of one for each row (fp32;
-    top_k int32 or int64) on the logits' device; numbers are used as fp32. Returns int64 tokens [...], and with
+    Each of temperature, top_k (a whole number), top_p and min_p is a number for all rows or a tensor [...] of one for each
+    row (fp32; top_k int32 or int64) on the logits' device; numbers are used as fp32. Returns int64 tokens [...], and with
     ``return_logprob`` also the fp32 log-probability of each token under the distribution it was drawn from. Weights
     and their sums are held in 64 bits: a token differs from the definition's only where u falls within about 1e-10 of a
     border between two. u = 0 gives the first index of any weight. No gradient."""

@@ -409,6 +409,29 @@ def test_shared_prefix_is_deterministic_and_row_independent():
         assert torch.equal(a, ops.shared_prefix_attention(*x.values(), lengths=lengths, prefix_lengths=pre))
 
 
+@pytest.mark.parametrize("n,Lq,P,S", [(20, 1, 3000, 90), (3, 24, 700, 150), (90, 1, 500, 30)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_shared_prefix_rows_do_not_touch_one_another(n, Lq, P, S, dtype):
+    """Other queries, own keys, values and lengths in all rows but one leave that row's bits as they are; so does another
+    prefix in the other group."""
+    x, lengths, pre = make(2, n, Lq, 6, 2, 128, P, S, dtype, True)
+    want = ops.shared_prefix_attention(*x.values(), lengths=lengths, prefix_lengths=pre)
+    for row in (0, n // 2, n, 2 * n - 1):
+        g = row // n
+        y, l2, p2 = make(2, n, Lq, 6, 2, 128, P, S, dtype, True, seed=50)
+        l2, p2 = l2.flip(0).contiguous(), p2.clone()
+        for name in ("k", "v"):
+            y[name] = y[name].nan_to_num()
+        for name in ("q", "k", "v"):
+            y[name][row] = x[name][row]
+        for name in ("pk", "pv"):
+            y[name][g] = x[name][g]
+        l2[row], p2[g] = lengths[row], pre[g]
+        got = ops.shared_prefix_attention(*y.values(), lengths=l2, prefix_lengths=p2)
+        assert torch.equal(got[row], want[row])
+        assert not torch.equal(got, want)
+
+
 # ----------------------------------------------------------------------------------------------------------------------
 # ways of calling
 
@@ -547,3 +570,46 @@ def test_generate_samples_native():
     assert out.shape == (8, prompt.shape[1] + 6) and bool((out[:, :prompt.shape[1]] == prompt).all())
     assert torch.equal(out, generate(m, prompt, tok, generator=gen(), **kw))
     assert bool((out[:, prompt.shape[1]] >= 0).all())
+
+
+@pytest.mark.parametrize("kw", [dict(top_p=0.95), dict(top_k=20, temperature=1.3), dict(min_p=0.02, top_k=40, top_p=0.9)])
+def test_generate_draws_the_definitions_tokens(kw, monkeypatch):
+    """Every token of a generation on the kernels is the 64-bit form's, for the logits that the model gave at that step, the
+    generator's next uniform numbers and the settings that were asked for."""
+    from faster_yoco_b200.config import build_args
+    from faster_yoco_b200.data.tokenizers import ByteTokenizer
+    from faster_yoco_b200.eval.generate import generate
+    from faster_yoco_b200.models.yoco import YOCO
+    torch.manual_seed(0)
+    with torch.device("cuda"):
+        m = YOCO(build_args("yoco_small", vocab_size=264, max_seq_len=512, max_batch_size=1))
+    m = m.to(torch.bfloat16).eval()
+    tok, n, steps = ByteTokenizer(), 8, 6
+    prompts = torch.tensor([tok.encode("x" * 300, bos=True), tok.encode("y" * 300, bos=True)], device="cuda")
+    P = prompts.shape[1]
+    kw = dict(dict(temperature=0.9), **kw)
+    given, plain = [], YOCO.forward
+
+    def forward(self, *a, **k):
+        out = plain(self, *a, **k)
+        if not k["is_prefilling"]:
+            given.append((a[0].clone(), out[0][:, -1].float()))
+        return out
+
+    monkeypatch.setattr(YOCO, "forward", forward)
+    out = generate(m, prompts, tok, generate_tokens=steps, chunk_length=128, num_samples=n,
+                   generator=torch.Generator(device="cuda").manual_seed(5), **kw)
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    N = 2 * n
+    pars = (rows_of(kw["temperature"], N, torch.float32), rows_of(kw.get("top_k", 0), N, torch.int64),
+            rows_of(kw.get("top_p", 1.0), N, torch.float32), rows_of(kw.get("min_p", 0.0), N, torch.float32))
+    ended = torch.zeros(N, dtype=torch.bool, device="cuda")
+    assert len(given) == steps or bool((out[:, P:] == tok.eos_id).any(1).all())
+    for i, (fed, logits) in enumerate(given):
+        assert torch.equal(fed[:, 0], out[:, P + i - 1])
+        logits[:, tok.bos_id] = logits[:, tok.pad_id] = -INF
+        want, _ = ref.sample(logits, torch.rand(N, generator=gen, device="cuda"), *pars)
+        want = torch.where(ended, torch.full_like(want, tok.pad_id), want)
+        assert torch.equal(out[:, P + i], want)
+        ended |= want == tok.eos_id
+    assert len({tuple(r.tolist()) for r in out[:n, P:]}) > 1
