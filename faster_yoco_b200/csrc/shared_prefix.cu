@@ -100,6 +100,15 @@ __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
   return *reinterpret_cast<uint32_t*>(&v);
 }
 
+// A mean of fp16 values lies within them. Weights rounded for the product (2^-11 of each, and the sums' 2^-19) can lift one at
+// the end of the range past it, where it would round to infinity; infinities and NaN stay.
+template <typename T>
+__device__ __forceinline__ float within_range(float x) {
+  constexpr float kMost = 65504.0f;
+  if (std::is_same<T, __half>::value && fabsf(x) < kMost * (1.0f + 0x1p-10f)) return fminf(fmaxf(x, -kMost), kMost);
+  return x;
+}
+
 // instruction descriptor of kind::f16 with fp32 accumulation; the format bits are 1 for bf16 and 0 for fp16
 template <typename T>
 __device__ __forceinline__ constexpr uint32_t idesc_of(int N, bool b_mn) {
@@ -706,7 +715,9 @@ __global__ void __launch_bounds__(kJoinCols * Parts * 32) spa_join_kernel(const 
       const float4 t = sO[q - 1][c4][lane & 7];
       x = make_float4(x.x + w[q] * t.x, x.y + w[q] * t.y, x.z + w[q] * t.z, x.w + w[q] * t.w);
     }
-    *reinterpret_cast<uint2*>(out + 4 * (c0 + c4)) = make_uint2(pack2<T>(x.x * inv, x.y * inv), pack2<T>(x.z * inv, x.w * inv));
+    *reinterpret_cast<uint2*>(out + 4 * (c0 + c4)) =
+        make_uint2(pack2<T>(within_range<T>(x.x * inv), within_range<T>(x.y * inv)),
+                   pack2<T>(within_range<T>(x.z * inv), within_range<T>(x.w * inv)));
   }
 }
 

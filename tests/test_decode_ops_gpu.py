@@ -395,6 +395,26 @@ def test_shared_prefix_nan_reaches_the_result(G, n, Lq, P, S, dtype):
                     assert torch.equal(got[~bad], want[~bad])
 
 
+@pytest.mark.parametrize("P,S", [(3, 1), (1, 3), (40, 7), (700, 20)])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_shared_prefix_largest_fp16_values(P, S, sign):
+    """A mean of values at the end of fp16's range is there too, whatever the rounding of its weights: random ones, and one
+    of 1 among many of 0.5 + 2^-12 + 2^-14, which fp16 rounds up by 0.75 2^-12, 1.5 half steps of the result."""
+    x, lengths, pre = make(1, 40, 1, 6, 2, 128, P, S, torch.float16, False)
+    for name in ("pv", "v"):
+        x[name].fill_(sign * torch.finfo(torch.float16).max)
+    check_attention(x, lengths, pre)
+    s = math.log(0.5 + 2.0 ** -12 + 2.0 ** -14)
+    coarse = float(torch.tensor(s).half())
+    x["q"].zero_()
+    x["q"][..., 0], x["q"][..., 1] = 1.0, 2.0 ** -6
+    for name in ("pk", "k"):
+        x[name].zero_()
+        x[name][..., 0], x[name][..., 1] = coarse, 64 * (s - coarse)
+    x["pk"][:, 0] = 0.0
+    check_attention(x, lengths, pre, scale=1.0)
+
+
 def test_shared_prefix_other_types():
     """fp32 and other head dims take the PyTorch expression."""
     for dtype, D in ((torch.float32, 128), (torch.float16, 32)):
