@@ -48,6 +48,7 @@ constexpr int kOwnBox = 32;             // key rows of one TMA box of own keys: 
 constexpr int kAtom = kT * 128;         // 128 rows of a 128-byte swizzle atom
 constexpr int kSpaThreads = 384;
 constexpr int kJoinCols = 2;            // warps of a joining block that share out the columns
+constexpr int kPieceTiles = 1 << 18;    // largest piece: 33 million keys against one block, a second
 constexpr float kRescaleLog2 = 8.0f;
 
 struct View {                           // [rows, keys, heads, D], last dim contiguous
@@ -840,6 +841,9 @@ at::Tensor shared_prefix_attention(const at::Tensor& q, const at::Tensor& pk, co
   for (int c = 0; c < 3; ++c) {
     const int units = std::min(total[c], c == 0 ? p.ctas : 2 * p.ctas);
     p.cuts[c] = units > 0 ? Cuts{units, total[c] / units, total[c] % units} : Cuts{0, 1, 0};
+    // the loader of the next query block waits for a whole piece: at up to 4 us a tile well within the limit of a wait
+    FYB_SUITS(std::min(p.cuts[c].len + 1, c == 2 ? p.tiles_o : p.tiles_p) <= kPieceTiles,
+              "shared_prefix_attention: too many keys for this many queries in one call");
   }
   p.shift = p.cuts[1].units % (2 * p.ctas);
   p.lengths = length_ptr(lengths, q, B, p.lengths_64);

@@ -534,6 +534,16 @@ def test_shared_prefix_refuses_scales_outside_fp32(scale):
         ops.shared_prefix_attention(*x.values(), lengths=lengths, prefix_lengths=pre, scale=scale)
 
 
+def test_shared_prefix_refuses_pieces_of_seconds():
+    """2^27 keys (overlapping rows of one buffer) against two blocks of queries an SM: each SM's share of one block would take
+    longer than the kernel's waits may. Refused before anything is launched."""
+    n = torch.cuda.get_device_properties(0).multi_processor_count * 256
+    pk = torch.zeros((1 << 27) * 8 + 128, device="cuda", dtype=torch.bfloat16).as_strided((1, 1 << 27, 1, 128), (8, 8, 8, 1))
+    q, own = (torch.zeros(n, s, 1, 128, device="cuda", dtype=torch.bfloat16) for s in (1, 0))
+    with pytest.raises(RuntimeError, match="too many keys"):
+        ops.shared_prefix_attention(q, pk, pk, own, own)
+
+
 @pytest.mark.parametrize("scale", [2.0 ** -126, 1e-30, 1e-3])
 def test_shared_prefix_small_scales(scale):
     x, lengths, pre = make(2, 4, 1, 6, 2, 128, 200, 50, torch.bfloat16, True)
