@@ -429,6 +429,36 @@ def test_shared_prefix_is_deterministic_and_row_independent():
         assert torch.equal(a, ops.shared_prefix_attention(*x.values(), lengths=lengths, prefix_lengths=pre))
 
 
+def test_offsets_beyond_32_bits():
+    """Rows, groups and positions 2^31 elements and more apart, in one buffer of 13 GB."""
+    far = (1 << 31) + 1024
+    buf = torch.zeros(3 * far, device="cuda", dtype=torch.bfloat16)
+    x, lengths, pre = make(3, 1, 2, 6, 2, 128, 300, 70, torch.bfloat16, True)
+
+    def spread(t, base, dim):                 # the steps along dim are `far`, everything else is dense
+        shape = list(t.shape)
+        shape[dim] = 1
+        strides = [shape[1] * shape[2] * shape[3], shape[2] * shape[3], shape[3], 1]
+        strides[dim] = far
+        y = buf[base:].as_strided(t.shape, strides)
+        return y.copy_(t)
+
+    base, got = 0, []
+    for name, t in x.items():
+        got.append(spread(t, base, 0))
+        base += 1 << 18
+    check_attention(x, lengths, pre, args=got)
+    one = dict(x, pk=x["pk"][:, :3], pv=x["pv"][:, :3], k=x["k"][:, :3], v=x["v"][:, :3])
+    got = [spread(t, i << 18, 1) for i, t in enumerate(one.values())]
+    check_attention(one, torch.tensor([3, 1, 2], device="cuda"), torch.tensor([2, 3, 1], device="cuda"), args=got)
+    logits = logits_like(3, 30011, torch.bfloat16, seed=8)
+    u = torch.rand(3, generator=torch.Generator(device="cuda").manual_seed(8), device="cuda")
+    y = buf[5:].as_strided(logits.shape, (far + 3, 1))
+    y.copy_(logits)
+    for kw in (dict(t=0.8, p=0.95), dict(k=50), dict(mp=0.01), dict(t=0.0)):
+        assert torch.equal(check_sample(y, u, **kw), check_sample(logits, u, **kw))
+
+
 @pytest.mark.parametrize("n,Lq,P,S", [(20, 1, 3000, 90), (3, 24, 700, 150), (90, 1, 500, 30)])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 def test_shared_prefix_rows_do_not_touch_one_another(n, Lq, P, S, dtype):
