@@ -257,13 +257,12 @@ __global__ void __launch_bounds__(kSpaThreads, 1)
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int cta = blockIdx.x;
-  if (threadIdx.x == 0) {
-    uint64_t* all = reinterpret_cast<uint64_t*>(bars);
-    for (int i = 0; i < static_cast<int>(sizeof(SpaBars) / 8); ++i) mbar_init(&all[i], 1);
-    for (int s = 0; s < 2; ++s) mbar_init(&bars->p_full[s], 4);
-    *abort_flag = 0;
+  if (threadIdx.x < sizeof(SpaBars) / 8) {   // a barrier a thread, each initialised once: p_full counts the four warps
+    uint64_t* bar = reinterpret_cast<uint64_t*>(bars) + threadIdx.x;
+    mbar_init(bar, bar == &bars->p_full[0] || bar == &bars->p_full[1] ? 4 : 1);
     fence_mbar_init();
   }
+  if (threadIdx.x == 0) *abort_flag = 0;
   if (warp == 1) {
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
