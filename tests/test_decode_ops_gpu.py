@@ -295,6 +295,21 @@ def test_shared_prefix(shape, dtype, ragged):
     check_attention(x, lengths, pre)
 
 
+# hundreds of groups of one row each (nothing shared), as many with prefixes of a few keys, a whole prompt of queries, the
+# fewest and the most heads a key / value head may have
+MORE_SHAPES = [(300, 1, 1, 6, 2, 128, 50, 20), (700, 1, 1, 4, 4, 64, 3, 1), (64, 1, 1, 24, 8, 128, 700, 130),
+               (1, 1, 1000, 6, 2, 128, 0, 1000), (2, 1, 300, 6, 2, 64, 200, 300), (40, 4, 2, 3, 3, 128, 129, 33),
+               (2, 1, 1, 640, 1, 64, 300, 40)]
+
+
+@pytest.mark.parametrize("shape", MORE_SHAPES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("ragged", [False, True])
+def test_shared_prefix_more_shapes(shape, dtype, ragged):
+    x, lengths, pre = make(*shape, dtype, ragged, seed=sum(shape))
+    check_attention(x, lengths, pre)
+
+
 @pytest.mark.parametrize("P,S", [(0, 0), (0, 5), (70, 0), (0, 300), (1, 0)])
 @pytest.mark.parametrize("n", [1, 60])
 def test_shared_prefix_empty_sides(P, S, n):
@@ -611,6 +626,35 @@ def test_sampled_generation_native():
             cur = ops.sample(a[:, -1], torch.rand(2 * n, device="cuda"), 1.0, 50, 0.95)[:, None]
     assert forked["prefix_key"].data_ptr() == one["prev_key"].data_ptr()
     assert forked["prev_key"].shape[1] < one["prev_key"].shape[1]
+
+
+def test_a_forked_state_outlives_what_its_parent_does_native():
+    """The kernels update the retention states and the K / V cache in place: what the parent does after a fork, behind the
+    prompt, inside it and over all of it, leaves the bits of the forked rows' logits as they are."""
+    from faster_yoco_b200.config import build_args
+    from faster_yoco_b200.models.yoco import YOCO
+    torch.manual_seed(0)
+    with torch.device("cuda"):
+        m = YOCO(build_args("yoco_small", vocab_size=264, max_seq_len=1024, max_batch_size=1))
+    m = m.to(torch.bfloat16).eval()
+    prompt, other = (torch.randint(3, 264, (2, 300), device="cuda") for _ in range(2))
+    for copies in (1, 3):
+        step = torch.randint(3, 264, (2 * copies, 1), device="cuda")
+
+        def decode(forked):
+            return torch.cat([m(step, incremental_state=forked, start_pos=300 + i, is_prefilling=False)[0] for i in range(3)])
+
+        with torch.no_grad():
+            state = {}
+            m(prompt, incremental_state=state, start_pos=0, is_prefilling=True, skip_cross_decoder=True)
+            want = decode(m.fork_state(state, 2, copies))
+            first, second, third = (m.fork_state(state, 2, copies) for _ in range(3))
+            m(prompt[:, :1], incremental_state=state, start_pos=300, is_prefilling=False)
+            assert torch.equal(decode(first), want)
+            m(prompt[:, :1], incremental_state=state, start_pos=200, is_prefilling=False)
+            assert torch.equal(decode(second), want)
+            m(other, incremental_state=state, start_pos=0, is_prefilling=True, skip_cross_decoder=True)
+            assert torch.equal(decode(third), want)
 
 
 def test_generate_samples_native():
