@@ -1,7 +1,7 @@
 // Sampling of one token for each row of logits from one uniform number a row: temperature, top-k, top-p, min-p.
 //
-// With w_i = exp((x_i - max) / T) the candidates, in descending order of x (ties: lowest index), are cut to the first k, to
-// the shortest prefix with at least p of the weight left and to w_i >= min_p; the token is the first kept index whose
+// With w_i = exp((x_i - max) / T) the candidates, in descending order of x (ties: lowest index), are cut to the first k,
+// to the shortest prefix with at least p of the weight left and to w_i >= min_p; the token is the first kept index whose
 // running weight in index order passes u times the kept weight.
 //
 // No sort of the vocabulary. A cluster of 1 to 8 CTAs has a row, each CTA a contiguous slice, each warp a contiguous
@@ -14,15 +14,20 @@
 //      usually a few hundred: one CTA ranks them in shared memory, cuts and draws.
 //   Otherwise the cut is found by a radix search over the order-preserving 32-bit image of the logits, with histograms of
 //   counts (top-k) or weights (top-p) in steps of 11 bits, and the draw goes by segment sums.
+//   A CTA's bound for top-k is its own slice's, so a row's list has at least CTAs x k candidates, of which it holds 512:
+//   with 8 CTAs (one or 16 rows of 100,288) k = 50 takes 21 and 32 us and k = 64 takes 85 and 122; with 4 (64 rows)
+//   k = 100 takes 39 and k = 128 takes 122; with one (256 rows) k = 200 takes 49 and k = 500 takes 223.
 //
 // Tokens are decided by comparing sums over the whole vocabulary, so weights are evaluated to 2^-48 in 64 bits and
 // summed in 64 bits: histograms as integers in a fixed point whose 62 bits the weight of all candidates fills, the rest in
 // floating point in a fixed order.
 //
-// Measured (B200): 64 rows of 100,288 bf16 logits, top-k and top-p, 22 us (0.6 TB/s; the read itself takes 2); 256 rows
-// without a filter 74 us, bound by the 64-bit exponentials (47 instructions a logit, 12 of them 64-bit at 60 a clock and
-// SM); one row with top-p 18 us, bound by cluster barriers (1.5 us each) and latency. CTAs a row at 64 rows: 1 / 2 / 4 / 8
-// take 29 / 24 / 22 / 53 us, at one row 53 / 37 / 26 / 18 us, at 400 rows 62 us with one and 152 with two.
+// Measured (B200): 64 rows of 100,288 bf16 logits, top-k and top-p, 23 us (0.6 TB/s; the read itself takes 2); 256 rows
+// without a filter 73 us, bound by the 64-bit exponentials (about 47 instructions a logit, 12 of them 64-bit at 60 a clock
+// and SM); one row with top-p 18 us, bound by cluster barriers (1.5 us each) and latency. CTAs a row at 64 rows: 1 / 2 /
+// 4 / 8 take 29 / 24 / 22 / 53 us, at one row 53 / 37 / 26 / 18 us, at 400 rows 62 us with one and 152 with two. A radix
+// row takes about 80 us on one CTA: 400 rows of 50,001 with settings of their own take 56 us, or 140 where such a row
+// starts last (two seeds of twelve).
 #include <ATen/ATen.h>
 #include <c10/util/Optional.h>
 #include <cooperative_groups.h>
@@ -78,9 +83,10 @@ __device__ __forceinline__ float value_of(uint32_t k) {
   return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);
 }
 
-// w = 2^(t / 32) for t = 32 log2(e) (x - max) / T <= 0, by a table of 2^(j / 32) and a polynomial on |r| <= 1/2 (the table-driven
-// method of P. T. P. Tang, 1989): 2^(r / 32) = 1 + r (c1 + r (c2 + ...)), c_i = (ln 2 / 32)^i / i!; the remainder after r^5 is
-// below 2^-48. The table lies in the lanes of the warp (lane j: 2^(j / 32)) and is read by shuffles: all lanes call.
+// w = 2^(t / 32) for t = 32 log2(e) (x - max) / T <= 0, by a table of 2^(j / 32) and a polynomial on |r| <= 1/2 (the
+// table-driven method of P. T. P. Tang, 1989): 2^(r / 32) = 1 + r (c1 + r (c2 + ...)), c_i = (ln 2 / 32)^i / i!; the
+// remainder after r^5 is below 2^-48. The table lies in the lanes of the warp (lane j: 2^(j / 32)) and is read by
+// shuffles: all lanes call.
 struct Weight {
   double top, scale, table;  // largest logit (finite), 32 log2(e) / T, this lane's 2^(lane / 32)
   float half, lowest;        // -max / 2; the (x - max) / 2 of a weight of 2^-1000

@@ -7,29 +7,38 @@
 // rows of ONE matrix product over the prefix, so its keys and values are read once for all of them; the own keys of each
 // row are a second, smaller product.
 //
-// Two kernels. spa_kernel, one persistent CTA an SM, walks 128-key tiles; spa_join_kernel joins the pieces. The tiles of all (group, head, 128-row block) are one line that is cut into equal ranges, so every SM
-// has the same number of tiles whatever the number of heads, and a piece is the part of one block's tiles that falls
-// into one range. Lengths are read on the device: ranges are cut from the stored sizes, tiles behind a length are
-// skipped.
+// Two kernels. spa_kernel, one persistent CTA an SM, walks 128-key tiles; spa_join_kernel joins the pieces. The tiles of
+// all (group, head, 128-row block) are one line that is cut into equal ranges, so every SM has the same number of tiles
+// whatever the number of heads, and a piece is the part of one block's tiles that falls into one range.
+//
+// Lengths are read on the device, so ranges are cut from the stored sizes and tiles behind a length are skipped: the SMs
+// share evenly what is stored, not what is in use. 32 rows on 4,096 keys take 26 us from a buffer of 4,096 and 37 from one
+// of 32,768; 1,000 keys 21 and 33; 16,384 keys 37 and 40.
+//
+// Scores, softmax statistics, sums and pieces are in fp32. The weights are rounded to the inputs' type for the product
+// with the values, as the tensor cores take both operands in one type: half a step of that type for each weight, on top of
+// the half step of the result. Against 64 bits a result errs by 2.2e-3 of its norm in bf16 and 2.8e-4 in fp16, where fp32
+// weights would give 1.7e-3 and 2.1e-4.
 //
 // Inside a CTA two streams of tiles run side by side, each with its own query block, scores S and output O in tensor
 // memory; one stream's softmax overlaps the other's products:
 //   warp 0      loads K / V tiles by TMA, in the order in which they are multiplied, into one ring of slots
-//   warp 1      issues S = Q K^T and O += P V (P, rounded to the inputs' type, over the first columns of S)
+//   warp 1      issues S = Q K^T and O += P V (P lies over the first columns of S)
 //   warps 2, 3  copy the query block of the next piece of stream 0 / 1 into shared memory (rows of any stride)
 //   warps 4-7, 8-11   softmax of stream 0 / 1, a thread a query row: running maximum (O is rescaled only when it grows
-//               by more than 2^8), exponentials, row sums in fp32, P back to tensor memory; at the end of a piece O, m, l
-//               to the workspace
+//               by more than 2^8), exponentials, row sums, P back to tensor memory; at the end of a piece O, m, l to the
+//               workspace
 // Work comes in three classes: (0) prefix blocks in pairs, both streams on the same K / V tile (compute bound: halves
 // the shared memory fills); (1) the odd last prefix block, each stream with tiles of its own; (2) own keys.
 //
-// Measured (B200, both kernels, bf16, 24 / 8 heads of 128): 32 rows on 16,384 shared keys with up to 256 of their own 37 us
-// (2.5 TB/s of what has to be read; the floor by bytes is 14), 128 rows on 32,768 + 512 138 us (378 TFLOP/s; floor 52), 20
-// x 24 queries on 2,000 + 24 40 us. What bounds it is neither memory nor the tensor cores (15 % busy) but the chain of a
-// tile: about 2,000 cycles of softmax (exponentials 1,024 at the rate of the SFUs, the rest latency of warps that run
-// alone) and 1,500 of products and hand-over, 4,800 a pair of tiles with two streams. Tried without gain: two threads a
-// row, four threads a row by copies of short blocks, an issuing warp for each stream, one pass over S, turns at the exponentials, rows of 64 or 128 columns in registers
-// (longer code: slower), launching the join ahead.
+// Measured (B200, both kernels, bf16, 24 / 8 heads of 128): 32 rows on 16,384 shared keys with up to 256 of their own
+// 37 us (2.5 TB/s of what has to be read; the floor by bytes is 14), 128 rows on 32,768 + 512 137 to 141 us (370 to 380
+// TFLOP/s; floor 52), 20 x 24 queries on 2,000 + 24 40 us. What bounds it is neither memory nor the tensor cores (15 to
+// 19 % busy) but the chain of a tile: about 2,000 cycles of softmax (exponentials 1,024 at the rate of the SFUs, the rest
+// latency of warps that run alone) and 1,500 of products and hand-over, 4,800 a pair of tiles with two streams. Tried
+// without gain: two threads a row, four threads a row by copies of short blocks, an issuing warp for each stream, one
+// pass over S, turns at the exponentials, rows of 64 or 128 columns in registers (longer code: slower), launching the join
+// ahead.
 #include <ATen/ATen.h>
 #include <c10/util/Optional.h>
 #include <cuda_fp16.h>
@@ -101,8 +110,8 @@ __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
   return *reinterpret_cast<uint32_t*>(&v);
 }
 
-// A mean of fp16 values lies within them. Weights rounded for the product (2^-11 of each, and the sums' 2^-19) can lift one at
-// the end of the range past it, where it would round to infinity; infinities and NaN stay.
+// A mean of fp16 values lies within them. Weights rounded for the product (2^-11 of each, and the sums' 2^-19) can lift
+// one at the end of the range past it, where it would round to infinity; infinities and NaN stay.
 template <typename T>
 __device__ __forceinline__ float within_range(float x) {
   constexpr float kMost = 65504.0f;
@@ -566,7 +575,7 @@ __global__ void __launch_bounds__(kSpaThreads, 1)
             tmem_ld_wait();
             hide(v, vis - c * 32);
 #pragma unroll
-            for (int j = 0; j < 16; ++j) {
+            for (int j = 0; j < 16; ++j) {        // l sums the weights as they are, P takes them rounded
               const float2 t = fma2(make_float2(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1])), sc, nm);
               const float2 e = make_float2(fast_exp2(t.x), fast_exp2(t.y));
               l2[j & 1] = add2(l2[j & 1], e);
@@ -618,9 +627,9 @@ __global__ void __launch_bounds__(kSpaThreads, 1)
 }
 
 // Joins the pieces of each output row: o = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i. A block has eight consecutive
-// rows of a (group, key / value head) and 1 / Split of their columns. Its warps share them out by columns (kJoinCols) and by
-// pieces (Parts); a lane has one row and some columns in fours, so that a load of a warp covers whole 128-byte lines and a
-// thread has its loads in flight together; the parts join in shared memory.
+// rows of a (group, key / value head) and 1 / Split of their columns. Its warps share them out by columns (kJoinCols) and
+// by pieces (Parts); a lane has one row and some columns in fours, so that a load of a warp covers whole 128-byte lines
+// and a thread has its loads in flight together; the parts join in shared memory.
 template <typename T, int D, int Parts, int Split>
 __global__ void __launch_bounds__(kJoinCols * Parts * 32) spa_join_kernel(const __grid_constant__ PrefixParams p) {
   constexpr int F = D / 4 / Split / (4 * kJoinCols);     // float4s of a lane: from c0 on, lane / 8 + 4 (wc + kJoinCols f)

@@ -29,8 +29,9 @@ def generate(model, prompt: torch.Tensor, tokenizer, generate_tokens: int = 20, 
              min_p: float = 0.0, generator: Optional[torch.Generator] = None) -> torch.Tensor:
     """prompt: [B, P] ids on the model's device -> [B * num_samples, P + generate_tokens] (pad where nothing was
     produced); rows b * num_samples .. (b + 1) * num_samples - 1 continue prompt b. temperature 0 is greedy; top_k,
-    top_p and min_p as in ``ops.sample``; generator: source of its uniform numbers (on the model's device; of tensor-parallel
-    ranks the first one's decide). A sampled row whose logits leave nothing to draw (all NaN or -inf) raises RuntimeError."""
+    top_p and min_p as in ``ops.sample``; generator: source of its uniform numbers (on the model's device; of
+    tensor-parallel ranks the first one's decide). A sampled row whose logits leave nothing to draw (all NaN or -inf)
+    raises RuntimeError."""
     if num_samples < 1 or not temperature >= 0:
         raise ValueError(f"generate: num_samples = {num_samples}, temperature = {temperature}")
     fork = num_samples > 1 and yoco and hasattr(model, "fork_state")

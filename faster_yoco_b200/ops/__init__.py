@@ -553,10 +553,14 @@ def shared_prefix_attention(q: torch.Tensor, prefix_k: torch.Tensor, prefix_v: t
     means all stored positions. Positions behind the lengths may hold anything. P, S, B or Lq may be 0; a query that
     sees no key gets zeros. scale: positive, default 1 / sqrt(D). Returns a contiguous [B, Lq, Hq, D].
 
-    The sm_100a kernel takes bf16 and fp16 with D 64 or 128 (and refuses a scale that is not normal in fp32); other types
-    and sizes run the PyTorch expression. Key / value tensors are read in place when their rows are 16-byte aligned, else
-    copied first. A NaN in a query, or in a key that it sees, makes its result NaN (as does a score of +inf). A value that SOME query of a
-    row sees has to be finite. Inference only."""
+    The sm_100a kernel takes bf16 and fp16 with D 64 or 128 (and refuses a scale that is not normal in fp32). It holds
+    scores, statistics and sums in fp32 and rounds the softmax weights to the inputs' type for the product with the values:
+    half a step of that type for each weight, besides the result's own. Other types and sizes run the PyTorch expression,
+    with fp32 weights. Key / value tensors are read in place when their rows are 16-byte aligned, else copied first. Work is
+    divided by the stored sizes P and S: lengths far below them leave part of the GPU idle.
+
+    A NaN in a query, or in a key that it sees, makes its result NaN (as does a score of +inf). A value that SOME query of a
+    row sees has to be finite, with weighted sums of values within fp32. Inference only."""
     _no_grad_op("shared_prefix_attention", q, prefix_k, prefix_v, k, v)
     scale = max(q.shape[-1], 1) ** -0.5 if scale is None else float(scale)
     if not 0.0 < scale < math.inf:

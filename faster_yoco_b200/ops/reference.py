@@ -232,8 +232,8 @@ def shared_prefix_attention(q, prefix_k, prefix_v, k, v, lengths=None, prefix_le
     """q: [B,Lq,Hq,D]; prefix_k / prefix_v: [G,P,Hk,D], shared by the B // G consecutive rows of each group;
     k / v: [B,S,Hk,D], the rows' own positions. Query i of row b sees prefix keys j < prefix_lengths[g] (default P) and
     own keys j <= lengths[b] - Lq + i, j < lengths[b] (default S; both clamped to what is stored). fp32 math; a
-    query that sees no key gets zeros, one that sees a score of NaN or +inf gets NaN. Values behind the lengths are not read
-    into the sums, whatever they hold."""
+    query that sees no key gets zeros, one that sees a score of NaN or +inf gets NaN. Values behind the lengths are not
+    read into the sums, whatever they hold."""
     B, Lq, Hq, D = q.shape
     G, P, Hk = prefix_k.shape[:3]
     S, n, rep, dev = k.shape[1], B // max(G, 1), Hq // Hk, q.device
